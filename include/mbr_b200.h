@@ -294,6 +294,113 @@ MBR_API int mbr_op_ffn(const void* d_x, const void* d_w1, const float* d_b1, con
 MBR_API int mbr_op_attention(const void* d_q, const void* d_k, const void* d_v, int64_t B, int heads, int N,
                              int dim_head, float scale, const float* d_gates, void* d_out, int dtype, void* stream);
 
+/* ---- streaming time-axis attention ----------------------------------------
+ * The attention of a layer whose frames arrive a few at a time, or of a track
+ * too long to attend over whole: per-head norms with rotary positions, a
+ * rolling key/value cache, and attention over a sliding window plus a few
+ * first tokens that stay visible.  The reference has no counterpart (its time
+ * axis attends over one whole chunk, src/mbr_cuda_tile.h:42-45); the pieces
+ * extend split_qkv_heads_rotary and scaled_dot_product_attention.
+ * All of these enqueue on `stream` and return without synchronising, allocate
+ * no device memory and may be captured into a CUDA graph (call the attention
+ * once before the capture: its first call on a device allocates one host-mapped
+ * word).  Calls on different streams are independent.  The device that is
+ * current at the call must own the buffers and the stream.  Tokens, heads or
+ * sequences of zero make a call that does nothing. */
+
+/* A [seqs][tokens][heads][dim_head] tensor read or written in place: element d
+ * of head h of token t of sequence s is data[s*seq + t*token + h*head + d]
+ * (strides in elements, any sign that stays inside the caller's buffer). */
+typedef struct mbr_view {
+    void* data;
+    int64_t seq, token, head;
+} mbr_view;
+
+/* A rolling key/value cache.  Position p of a sequence lives in slot p while
+ * p < sinks and in slot sinks + (p - sinks) % ring after that, so the first
+ * `sinks` tokens stay and the newest `ring` others replace the older ones.
+ * bits 0: k and v are [seqs][kv_heads][sinks + ring][dim_head] of dtype
+ * (MBR_FP32 / MBR_FP16 / MBR_BF16), k_scale and v_scale are null.
+ * bits 4 (MBR_FP16 / MBR_BF16, dim_head a multiple of 32): k and v hold one
+ * byte for two values, channel 2i in the low half of byte i; k_scale and
+ * v_scale are [seqs][kv_heads][sinks + ring][dim_head / 32][2] of dtype, the
+ * step s and offset m of each group of 32 channels: code c stands for
+ * m + s * (c - 8), rounded to dtype. */
+typedef struct mbr_kv_cache {
+    void* k;
+    void* v;
+    void* k_scale;
+    void* v_scale;
+    int64_t seqs;
+    int kv_heads, dim_head;
+    int sinks, ring;
+    int dtype, bits;
+} mbr_kv_cache;
+
+/* Norm of every query and key over its head and rotary positions, in one pass:
+ * y = x * rsqrt(mean_d x^2 + eps) * gamma, then pair (2i, 2i+1) of the axis a
+ * that owns pair i turned by (d_cos, d_sin)[d_pos[s][t][a]][i] (tables
+ * [table_rows][dim_head / 2] fp32, e.g. mbr_rope_tables).  h_pairs[axes] (host)
+ * are the pairs of each axis, in order; pairs after the last section are normed
+ * but not turned, axes 0 turns none.  A position outside [0, table_rows) makes
+ * that axis' pairs NaN.  q [.. q_heads ..], k [.. kv_heads ..] of dtype, gamma
+ * fp32 [dim_head] or null (ones); outputs may be the inputs (in place) or
+ * buffers that do not overlap them.  dim_head even, 2..256; axes 0..4; k and
+ * k_out may be null with kv_heads 0.
+ * Extends the rotary part of split_qkv_heads_rotary (src/mbr_cuda_tile.h:8-10). */
+MBR_API int mbr_op_qk_norm_rope(const mbr_view* q, const mbr_view* k, const mbr_view* q_out, const mbr_view* k_out,
+                                int64_t seqs, int64_t tokens, int q_heads, int kv_heads, int dim_head,
+                                const float* d_gamma_q, const float* d_gamma_k, float eps, const float* d_cos,
+                                const float* d_sin, int64_t table_rows, const int32_t* d_pos, int axes,
+                                const int* h_pairs, int dtype, void* stream);
+
+/* Writes tokens d_pos[s] + i, i < d_count[s] (null: tokens; more than `tokens`
+ * counts as `tokens`), into the cache; k, v [seqs][tokens][kv_heads][dim_head].
+ * Of tokens that share a ring slot only the newest is written; negative
+ * positions are left out.  4-bit groups: with T(x) the rounding to dtype, s =
+ * T((max - min) / 15), m = T(min + 8 s), c = clamp(rint((x - m) / s) + 8, 0,
+ * 15); a group whose range is not finite is NaN when read. */
+MBR_API int mbr_op_cache_append(const mbr_kv_cache* cache, const mbr_view* k, const mbr_view* v,
+                                const int32_t* d_pos, const int32_t* d_count, int64_t tokens, void* stream);
+
+/* Reads positions d_pos[s] + i, i < d_count[s], of a cache whose newest token
+ * is the last of them, as dtype values (the values that 4-bit codes stand
+ * for); positions that the cache no longer holds, negative ones and i >=
+ * d_count[s] read as zeros. */
+MBR_API int mbr_op_cache_read(const mbr_kv_cache* cache, const int32_t* d_pos, const int32_t* d_count,
+                              int64_t tokens, const mbr_view* k, const mbr_view* v, void* stream);
+
+/* Attention of many queries over a sliding window and the first tokens:
+ * out[s][i][h] = gate * sum_j softmax_j(scale q.k_j) v_j over the keys j in
+ * [0, kv_len[s]) with j <= p + right and (j >= p - left or j < sinks), p =
+ * kv_len[s] - q_len[s] + i the position of query i (the queries are the last
+ * tokens of the keys).  left / right < 0: no limit on that side.  Query head h
+ * reads key head h / (q_heads / kv_heads).  d_q_len, d_kv_len [seqs] (device)
+ * may be null (all q_tokens / kv_tokens) and are clamped to those; rows i >=
+ * q_len[s] and rows that see no key are zeros.  Keys that a query does not see
+ * have no effect on it, whatever they hold.  scale 0 means 1/sqrt(dim_head);
+ * d_gates [seqs][q_tokens][q_heads] fp32 or null.  dim_head a multiple of 8 up
+ * to 128.
+ * fp16/bf16 run on the tensor cores when pointers and strides are multiples of
+ * 16 bytes; other layouts and fp32 on the CUDA cores.  The first call after a
+ * kernel-side wait ran out returns MBR_ERR_TIMEOUT. */
+MBR_API int mbr_op_window_attention(const mbr_view* q, const mbr_view* k, const mbr_view* v, const mbr_view* out,
+                                    int64_t seqs, int64_t q_tokens, int64_t kv_tokens, int q_heads, int kv_heads,
+                                    int dim_head, const int32_t* d_q_len, const int32_t* d_kv_len, int left,
+                                    int right, int sinks, float scale, const float* d_gates, int dtype,
+                                    void* stream);
+
+/* The same attention for the newest `tokens` tokens over a cache that holds
+ * them already: d_length[s] tokens have been appended to sequence s, query i
+ * has position d_length[s] - tokens + i (rows of negative position are zeros)
+ * and sees the cached positions j <= p + right with j >= p - left or j <
+ * cache->sinks.  Cached means j < sinks or j >= d_length[s] - ring.  q, out
+ * [seqs][tokens][q_heads][dim_head] of the cache's dtype, d_gates
+ * [seqs][tokens][q_heads] fp32 or null. */
+MBR_API int mbr_op_cache_attention(const mbr_view* q, const mbr_kv_cache* cache, const mbr_view* out,
+                                   const int32_t* d_length, int64_t tokens, int q_heads, int left, int right,
+                                   float scale, const float* d_gates, void* stream);
+
 /* Host tables of MelBandRoformer::compute_rotary_cos_sin
  * (src/model_mel_band_roformer.cu:270-300): h_cos, h_sin [L][dim_head/2]. */
 MBR_API int mbr_rope_tables(int L, int dim_head, float* h_cos, float* h_sin);

@@ -15,6 +15,7 @@
 #include "audio_io.h"
 #include "ops_api.h"
 #include "separator.h"
+#include "stream_ops.h"
 #include "weights.h"
 
 struct mbr_handle {
@@ -580,6 +581,64 @@ MBR_API int mbr_op_attention(const void* d_q, const void* d_k, const void* d_v, 
         if (B > 0)
             mbr::opsapi::attention(d_q, d_k, d_v, B, heads, N, dim_head, scale, d_gates, d_out, dtype,
                                    (cudaStream_t)stream);
+    });
+}
+
+// ---- streaming time-axis attention ----
+namespace {
+// A view argument: null is an empty view (allowed where nothing is read or written).
+mbr_view view_or_empty(const mbr_view* v) { return v ? *v : mbr_view{}; }
+}  // namespace
+
+MBR_API int mbr_op_qk_norm_rope(const mbr_view* q, const mbr_view* k, const mbr_view* q_out, const mbr_view* k_out,
+                                int64_t seqs, int64_t tokens, int q_heads, int kv_heads, int dim_head,
+                                const float* d_gamma_q, const float* d_gamma_k, float eps, const float* d_cos,
+                                const float* d_sin, int64_t table_rows, const int32_t* d_pos, int axes,
+                                const int* h_pairs, int dtype, void* stream) {
+    return guard([&] {
+        mbr::streamops::qk_norm_rope(view_or_empty(q), view_or_empty(k), view_or_empty(q_out), view_or_empty(k_out),
+                                     seqs, tokens, q_heads, kv_heads, dim_head, d_gamma_q, d_gamma_k, eps, d_cos,
+                                     d_sin, table_rows, d_pos, axes, h_pairs, dtype, (cudaStream_t)stream);
+    });
+}
+
+MBR_API int mbr_op_cache_append(const mbr_kv_cache* cache, const mbr_view* k, const mbr_view* v,
+                                const int32_t* d_pos, const int32_t* d_count, int64_t tokens, void* stream) {
+    return guard([&] {
+        need(cache, "null argument");
+        mbr::streamops::cache_append(*cache, view_or_empty(k), view_or_empty(v), d_pos, d_count, tokens,
+                                     (cudaStream_t)stream);
+    });
+}
+
+MBR_API int mbr_op_cache_read(const mbr_kv_cache* cache, const int32_t* d_pos, const int32_t* d_count,
+                              int64_t tokens, const mbr_view* k, const mbr_view* v, void* stream) {
+    return guard([&] {
+        need(cache, "null argument");
+        mbr::streamops::cache_read(*cache, d_pos, d_count, tokens, view_or_empty(k), view_or_empty(v),
+                                   (cudaStream_t)stream);
+    });
+}
+
+MBR_API int mbr_op_window_attention(const mbr_view* q, const mbr_view* k, const mbr_view* v, const mbr_view* out,
+                                    int64_t seqs, int64_t q_tokens, int64_t kv_tokens, int q_heads, int kv_heads,
+                                    int dim_head, const int32_t* d_q_len, const int32_t* d_kv_len, int left,
+                                    int right, int sinks, float scale, const float* d_gates, int dtype,
+                                    void* stream) {
+    return guard([&] {
+        mbr::streamops::window_attention(view_or_empty(q), view_or_empty(k), view_or_empty(v), view_or_empty(out),
+                                         seqs, q_tokens, kv_tokens, q_heads, kv_heads, dim_head, d_q_len, d_kv_len,
+                                         left, right, sinks, scale, d_gates, dtype, (cudaStream_t)stream);
+    });
+}
+
+MBR_API int mbr_op_cache_attention(const mbr_view* q, const mbr_kv_cache* cache, const mbr_view* out,
+                                   const int32_t* d_length, int64_t tokens, int q_heads, int left, int right,
+                                   float scale, const float* d_gates, void* stream) {
+    return guard([&] {
+        need(cache, "null argument");
+        mbr::streamops::cache_attention(view_or_empty(q), *cache, view_or_empty(out), d_length, tokens, q_heads, left,
+                                        right, scale, d_gates, (cudaStream_t)stream);
     });
 }
 

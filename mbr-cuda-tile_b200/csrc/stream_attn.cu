@@ -1,0 +1,96 @@
+// stream_attn.cu — entry points of the streaming attention (prompt form and
+// few-token form over the rolling cache) and the warp-per-row kernel.
+#include <algorithm>
+#include <cmath>
+
+#include "stream_attn.cuh"
+
+namespace mbr {
+namespace streamops {
+
+namespace {
+
+// One warp per row: right for every layout and type.
+template <typename T, bool CACHED, bool Q4>
+__global__ void __launch_bounds__(256) attend_rows_kernel(const AttnArgs a) {
+    const int64_t rows = a.seqs * a.Nq * a.Hq, step = (int64_t)gridDim.x * 8;
+    for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += step) {
+        const int64_t si = r / a.Hq, s = si / a.Nq;
+        int n, m;
+        lengths<CACHED>(a, s, n, m);
+        attend_row<T, CACHED, Q4>(a, s, (int)(si - s * a.Nq), (int)(r - si * a.Hq), n, m);
+    }
+}
+
+template <bool CACHED>
+void launch_rows(const AttnArgs& a, int dtype, bool q4, cudaStream_t st) {
+    const int64_t rows = a.seqs * a.Nq * a.Hq;
+    const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(rows, 8), 148 * 64);
+    MBR_DISPATCH_DTYPE(dtype, T, {
+        if constexpr (CACHED && !std::is_same_v<T, float>) {
+            if (q4) {
+                attend_rows_kernel<T, true, true><<<grid, 256, 0, st>>>(a);
+                MBR_CUDA(cudaGetLastError());
+                return;
+            }
+        }
+        attend_rows_kernel<T, CACHED, false><<<grid, 256, 0, st>>>(a);
+    });
+    MBR_CUDA(cudaGetLastError());
+}
+
+// A limit of 2^30 or more is none (keys number fewer).
+int limit(int v) { return v >= (1 << 30) ? -1 : v; }
+
+AttnArgs common_args(const mbr_view& q, const mbr_view& out, int64_t seqs, int64_t Nq, int Hq, int Hkv, int D,
+                     int left, int right, int sinks, float scale, const float* gates) {
+    MBR_CHECK(seqs >= 0 && Nq >= 0 && Hq >= 0 && Hkv >= 0, "attention: negative size");
+    MBR_CHECK(D >= 8 && D <= 128 && D % 8 == 0, "attention: dim_head must be a multiple of 8 up to 128");
+    MBR_CHECK(Hkv == 0 ? Hq == 0 : Hq % Hkv == 0, "attention: q_heads must be a multiple of kv_heads");
+    MBR_CHECK(Nq < (1 << 30) && Hq < (1 << 20), "attention: too many queries or heads");
+    MBR_CHECK(seqs <= ((int64_t)1 << 40) / std::max<int64_t>(1, Nq * Hq), "attention: too many rows");
+    MBR_CHECK(std::isfinite(scale), "attention: scale must be finite");
+    AttnArgs a{};
+    a.q = q.data, a.out = out.data;
+    a.q_seq = q.seq, a.q_tok = q.token, a.q_head = q.head;
+    a.o_seq = out.seq, a.o_tok = out.token, a.o_head = out.head;
+    a.seqs = seqs, a.Nq = (int)Nq, a.Hq = Hq, a.Hkv = Hkv, a.D = D, a.G = Hkv ? Hq / Hkv : 1;
+    a.left = limit(left), a.right = limit(right), a.sinks = sinks;
+    a.scale = scale == 0.f ? 1.f / std::sqrt((float)D) : scale;
+    a.gates = gates;
+    return a;
+}
+
+}  // namespace
+
+void window_attention(const mbr_view& q, const mbr_view& k, const mbr_view& v, const mbr_view& out, int64_t seqs,
+                      int64_t Nq, int64_t Nk, int Hq, int Hkv, int D, const int32_t* q_len, const int32_t* kv_len,
+                      int left, int right, int sinks, float scale, const float* gates, int dtype, cudaStream_t st) {
+    AttnArgs a = common_args(q, out, seqs, Nq, Hq, Hkv, D, left, right, sinks, scale, gates);
+    MBR_CHECK(Nk >= 0 && Nk < (1 << 30) && sinks >= 0, "window_attention: bad key count or sinks");
+    MBR_CHECK(dtype == DT_F32 || dtype == DT_F16 || dtype == DT_BF16,
+              "window_attention: dtype must be fp32, fp16 or bf16");
+    if (seqs == 0 || Nq == 0 || Hq == 0) return;
+    MBR_CHECK(q.data && out.data && (Nk == 0 || (k.data && v.data)), "window_attention: null buffer");
+    a.Nk = (int)Nk;
+    a.k = k.data, a.v = v.data;
+    a.k_seq = k.seq, a.k_tok = k.token, a.k_head = k.head;
+    a.v_seq = v.seq, a.v_tok = v.token, a.v_head = v.head;
+    a.q_len = q_len, a.kv_len = kv_len;
+    launch_rows<false>(a, dtype, false, st);
+}
+
+void cache_attention(const mbr_view& q, const mbr_kv_cache& c, const mbr_view& out, const int32_t* length,
+                     int64_t tokens, int Hq, int left, int right, float scale, const float* gates, cudaStream_t st) {
+    const bool q4 = check_cache(c);
+    AttnArgs a = common_args(q, out, c.seqs, tokens, Hq, c.kv_heads, c.dim_head, left, right, c.sinks, scale, gates);
+    if (c.seqs == 0 || tokens == 0 || Hq == 0) return;
+    MBR_CHECK(q.data && out.data && length, "cache_attention: null buffer");
+    a.k = c.k, a.v = c.v, a.k_scale = c.k_scale, a.v_scale = c.v_scale;
+    a.ring = c.ring, a.cache_sinks = c.sinks, a.slots = (int64_t)c.sinks + c.ring;
+    a.kv_len = length;
+    launch_rows<true>(a, c.dtype, q4, st);
+}
+
+}  // namespace streamops
+}  // namespace mbr

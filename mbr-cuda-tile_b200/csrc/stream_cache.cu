@@ -1,0 +1,155 @@
+// stream_cache.cu — writing tokens to the rolling key/value cache and reading
+// them back, 16/32-bit rows or 4-bit codes with a step and an offset per 32
+// channels.  Both move each byte once; memory (or, for a single frame, the
+// launch) bounds them.
+#include <algorithm>
+
+#include "stream_cache.cuh"
+
+namespace mbr {
+namespace streamops {
+
+bool check_cache(const mbr_kv_cache& c) {
+    MBR_CHECK(c.seqs >= 0 && c.kv_heads >= 0 && c.sinks >= 0, "kv cache: negative size");
+    MBR_CHECK(c.ring >= 1 && c.sinks < (1 << 30) && c.ring < (1 << 30), "kv cache: ring must be 1..2^30 - 1");
+    MBR_CHECK(c.dtype == DT_F32 || c.dtype == DT_F16 || c.dtype == DT_BF16, "kv cache: dtype must be fp32, fp16 or bf16");
+    MBR_CHECK(c.bits == 0 || c.bits == 4, "kv cache: bits must be 0 or 4");
+    MBR_CHECK(c.dim_head >= 8 && c.dim_head <= 128 && c.dim_head % 8 == 0,
+              "kv cache: dim_head must be a multiple of 8 up to 128");
+    const bool some = c.seqs > 0 && c.kv_heads > 0;
+    MBR_CHECK(!some || (c.k && c.v), "kv cache: null buffer");
+    MBR_CHECK((((uintptr_t)c.k | (uintptr_t)c.v) & 15) == 0, "kv cache: buffers must be 16-byte aligned");
+    if (c.bits == 4) {
+        MBR_CHECK(c.dtype != DT_F32 && c.dim_head % kGroup == 0,
+                  "kv cache: 4 bits need fp16 or bf16 and dim_head a multiple of 32");
+        MBR_CHECK(!some || (c.k_scale && c.v_scale), "kv cache: 4 bits need the steps and offsets");
+        MBR_CHECK((((uintptr_t)c.k_scale | (uintptr_t)c.v_scale) & 15) == 0, "kv cache: buffers must be 16-byte aligned");
+    }
+    MBR_CHECK(!some || c.seqs <= ((int64_t)1 << 40) / c.kv_heads / ((int64_t)c.sinks + c.ring), "kv cache: too large");
+    return c.bits == 4;
+}
+
+namespace {
+
+struct RowArgs {
+    mbr_kv_cache c;
+    mbr_view k, v;
+    const int32_t *pos, *count;
+    int64_t tokens, rows;  // rows: seqs * tokens * kv_heads
+};
+
+// The row (sequence, token, head) of index r, its position and cache row; held:
+// it is (append: will be) in the cache.
+struct Row {
+    int64_t s, t, slot_row;
+    int h;
+    bool held;
+};
+__device__ __forceinline__ Row row_of(const RowArgs& a, int64_t r) {
+    Row w;
+    const int64_t st = r / a.c.kv_heads;
+    w.h = (int)(r - st * a.c.kv_heads);
+    w.s = st / a.tokens;
+    w.t = st - w.s * a.tokens;
+    const int64_t n = a.count ? min((int64_t)max(a.count[w.s], 0), a.tokens) : a.tokens;
+    const int64_t p0 = a.pos[w.s], p = p0 + w.t, last = p0 + n - 1;
+    w.held = w.t < n && p >= 0 && p <= INT32_MAX && (p < a.c.sinks || p > last - a.c.ring);
+    const int64_t slots = (int64_t)a.c.sinks + a.c.ring;
+    w.slot_row = (w.s * a.c.kv_heads + w.h) * slots + (w.held ? slot_of((int)p, a.c.sinks, a.c.ring) : 0);
+    return w;
+}
+
+template <typename T>
+__device__ __forceinline__ const T* at(const mbr_view& v, const Row& w) {
+    return (const T*)v.data + w.s * v.seq + w.t * v.token + w.h * v.head;
+}
+
+// One warp per (token, head): lane l holds channels l, l + 32, ...
+template <typename T, bool Q4, bool READ>
+__global__ void __launch_bounds__(256) cache_rows_kernel(const RowArgs a) {
+    const int lane = threadIdx.x & 31, D = a.c.dim_head;
+    const int64_t step = (int64_t)gridDim.x * 8;
+    for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < a.rows; r += step) {
+        const Row w = row_of(a, r);
+        if (!READ && !w.held) continue;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+            T* x = const_cast<T*>(at<T>(kv ? a.v : a.k, w));
+            void* data = kv ? a.c.v : a.c.k;
+            T* scale = (T*)(kv ? a.c.v_scale : a.c.k_scale);
+            for (int c = 0; c * 32 < D; ++c) {
+                const int d = c * 32 + lane;
+                if (!Q4) {
+                    T* row = (T*)data + w.slot_row * D;
+                    if (d < D) {
+                        if (READ) x[d] = w.held ? row[d] : from_f32<T>(0.f);
+                        else row[d] = x[d];
+                    }
+                } else {  // D % 32 == 0: one group
+                    uint8_t* row = (uint8_t*)data + w.slot_row * (D / 2);
+                    T* sm = scale + (w.slot_row * (D / kGroup) + c) * 2;
+                    if (READ) {
+                        const int code = (row[d >> 1] >> ((d & 1) * 4)) & 15;
+                        x[d] = w.held ? code_value<T>(code, to_f32<T>(sm[0]), to_f32<T>(sm[1])) : from_f32<T>(0.f);
+                    } else {
+                        const float v = to_f32<T>(x[d]);
+                        float lo = v, hi = v;
+#pragma unroll
+                        for (int o = 16; o > 0; o >>= 1) {
+                            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+                            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+                        }
+                        const bool ok = __all_sync(0xffffffffu, isfinite(v)) && isfinite(hi - lo);
+                        const T sT = from_f32<T>(__fmul_rn(hi - lo, 1.f / 15.f));
+                        const float s = to_f32<T>(sT);
+                        const T mT = from_f32<T>(__fadd_rn(lo, 8.f * s));
+                        const float m = to_f32<T>(mT), inv = s > 0.f ? __frcp_rn(s) : 0.f;
+                        const float q = rintf(__fmul_rn(__fadd_rn(v, -m), inv)) + 8.f;
+                        int code = (int)fminf(fmaxf(q, 0.f), 15.f);
+                        const int other = __shfl_down_sync(0xffffffffu, code, 1);
+                        if ((lane & 1) == 0) row[d >> 1] = (uint8_t)(code | (other << 4));
+                        if (lane == 0) {
+                            sm[0] = ok ? sT : from_f32<T>(NAN);
+                            sm[1] = ok ? mT : from_f32<T>(NAN);
+                        }
+                    }
+                }
+            }
+        }
+    }
+}
+
+template <bool READ>
+void run(const mbr_kv_cache& c, const mbr_view& k, const mbr_view& v, const int32_t* pos, const int32_t* count,
+         int64_t tokens, cudaStream_t st) {
+    const bool q4 = check_cache(c);
+    MBR_CHECK(tokens >= 0, "kv cache: negative token count");
+    if (c.seqs == 0 || c.kv_heads == 0 || tokens == 0) return;
+    MBR_CHECK(k.data && v.data && pos, "kv cache: null buffer");
+    MBR_CHECK(tokens < (1 << 30) && c.seqs <= ((int64_t)1 << 50) / tokens / c.kv_heads, "kv cache: too many rows");
+    RowArgs a{c, k, v, pos, count, tokens, c.seqs * tokens * c.kv_heads};
+    const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(a.rows, 8), 148 * 64);
+    MBR_DISPATCH_DTYPE(c.dtype, T, {
+        if constexpr (std::is_same_v<T, float>) {
+            cache_rows_kernel<T, false, READ><<<grid, 256, 0, st>>>(a);
+        } else {
+            if (q4) cache_rows_kernel<T, true, READ><<<grid, 256, 0, st>>>(a);
+            else cache_rows_kernel<T, false, READ><<<grid, 256, 0, st>>>(a);
+        }
+    });
+    MBR_CUDA(cudaGetLastError());
+}
+
+}  // namespace
+
+void cache_append(const mbr_kv_cache& c, const mbr_view& k, const mbr_view& v, const int32_t* pos,
+                  const int32_t* count, int64_t tokens, cudaStream_t st) {
+    run<false>(c, k, v, pos, count, tokens, st);
+}
+void cache_read(const mbr_kv_cache& c, const int32_t* pos, const int32_t* count, int64_t tokens, const mbr_view& k,
+                const mbr_view& v, cudaStream_t st) {
+    run<true>(c, k, v, pos, count, tokens, st);
+}
+
+}  // namespace streamops
+}  // namespace mbr

@@ -1,0 +1,43 @@
+// stream_cache.cuh — device view of the rolling key/value cache: slot of a
+// position, the values of a 4-bit row, and which keys a query sees.
+#pragma once
+
+#include "common.cuh"
+#include "stream_ops.h"
+
+namespace mbr {
+namespace streamops {
+
+constexpr int kGroup = 32;  // channels that share a step and an offset in a 4-bit cache
+
+// Slot of position p >= 0.
+__device__ __forceinline__ int64_t slot_of(int p, int sinks, int ring) {
+    return p < sinks ? p : sinks + (int64_t)((unsigned)(p - sinks) % (unsigned)ring);
+}
+
+// The value that code c of a group with step s and offset m stands for: exact
+// in fp32 (a 4-bit integer times a 16-bit value) up to the sum's rounding,
+// then rounded to the cache's type.
+template <typename T>
+__device__ __forceinline__ T code_value(int c, float s, float m) {
+    return from_f32<T>(m + s * (float)(c - 8));
+}
+
+// Keys of a query at position p over `len` keys: [lo, hi) and [0, first).
+// left / right < 0: no limit.  No sum here leaves 32 bits: p >= 0 or right <
+// 2^30 (the host turns larger limits into "none").
+struct Window {
+    int lo, hi, first;
+};
+__device__ __forceinline__ Window window_of(int p, int len, int left, int right, int sinks) {
+    Window w;
+    w.hi = right < 0 || (p >= 0 && right >= len - p) ? len : min(len, p + right + 1);
+    w.hi = max(w.hi, 0);
+    w.lo = left < 0 ? 0 : max(0, p - left);
+    w.lo = min(w.lo, w.hi);
+    w.first = min(min(sinks, w.hi), w.lo);
+    return w;
+}
+
+}  // namespace streamops
+}  // namespace mbr

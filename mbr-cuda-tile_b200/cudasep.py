@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 import numpy as np
 
@@ -30,6 +31,8 @@ EXPORTS = [
     "mbr_shard_run", "mbr_shard_window", "mbr_plan_shard_window", "mbr_shard_run_window", "mbr_shard_add_boundary", "mbr_shard_finalize", "mbr_set_graphs", "mbr_set_backend", "mbr_last_launches",
     "mbr_sync_check", "mbr_profile_enable", "mbr_profile_read",
     "mbr_op_rms_norm", "mbr_op_add", "mbr_op_gelu", "mbr_op_sigmoid_gate", "mbr_op_rope", "mbr_op_attention", "mbr_op_linear", "mbr_op_ffn",
+    "mbr_op_qk_norm_rope", "mbr_op_cache_append", "mbr_op_cache_read", "mbr_op_window_attention",
+    "mbr_op_cache_attention",
     "mbr_rope_tables",
     "mbr_op_band_gather", "mbr_op_mask_scatter", "mbr_op_stft", "mbr_op_istft", "mbr_op_istft_noalloc",
     "mbr_plan_shard", "mbr_wav_info", "mbr_wav_read", "mbr_wav_write",
@@ -92,6 +95,13 @@ def lib():
         L.mbr_op_linear.argtypes = [fp, fp, fp, fp, i64, c_int, c_int, c_int, c_int, vp]
         L.mbr_op_attention.argtypes = [fp, fp, fp, i64, c_int, c_int, c_int, c_float, fp, fp, c_int, vp]
         L.mbr_op_ffn.argtypes = [fp, fp, fp, fp, fp, fp, i64, c_int, c_int, c_int, vp]
+        L.mbr_op_qk_norm_rope.argtypes = [vp, vp, vp, vp, i64, i64, c_int, c_int, c_int, fp, fp, c_float, fp, fp, i64,
+                                          vp, c_int, vp, c_int, vp]
+        L.mbr_op_cache_append.argtypes = [vp, vp, vp, vp, vp, i64, vp]
+        L.mbr_op_cache_read.argtypes = [vp, vp, vp, i64, vp, vp, vp]
+        L.mbr_op_window_attention.argtypes = [vp, vp, vp, vp, i64, i64, i64, c_int, c_int, c_int, vp, vp, c_int, c_int,
+                                              c_int, c_float, fp, c_int, vp]
+        L.mbr_op_cache_attention.argtypes = [vp, vp, vp, vp, i64, c_int, c_int, c_int, c_float, fp, vp]
         L.mbr_rope_tables.argtypes = [c_int, c_int, fp, fp]
         L.mbr_op_band_gather.argtypes = [vp, fp, c_int, c_int, fp, c_int, vp]
         L.mbr_op_mask_scatter.argtypes = [vp, fp, fp, c_int, c_int, c_int, fp, c_int, vp]
@@ -226,6 +236,232 @@ def op_attention(q, k, v, scale=0.0, gates=None, out=None, stream=None):
     g = _ptr(gates) if gates is not None else None
     _check(lib().mbr_op_attention(_ptr(q), _ptr(k), _ptr(v), B, H, N, D, float(scale), g, _ptr(out), _dt(q),
                                   _stream(stream)))
+    return out
+
+
+# ---- streaming time-axis attention ----
+_VIEW = struct.Struct("@Pqqq")  # mbr_view
+_CACHE = struct.Struct("@PPPPqiiiiii")  # mbr_kv_cache
+
+
+def _view(t) -> bytes:
+    """mbr_view of a [seqs, tokens, heads, dim_head] tensor."""
+    a, b, c, _ = t.stride()
+    return _VIEW.pack(t.data_ptr(), a, b, c)
+
+
+def _need(cond, msg):
+    if not cond:
+        raise ValueError(msg)
+
+
+def _need_rows(device, dtype, **tensors):
+    """Every tensor is [seqs, tokens, heads, dim_head] of `dtype` on `device` with its last axis contiguous."""
+    for name, t in tensors.items():
+        if t.dim() != 4 or t.dtype != dtype or t.device != device or (t.shape[3] > 1 and t.stride(3) != 1):
+            raise ValueError(f"{name} must be [seqs, tokens, heads, dim_head] of {dtype} on {device} with a contiguous "
+                             f"last axis, got {tuple(t.shape)} of {t.dtype} on {t.device}")
+
+
+def _need_flat(device, dtype, shape, **tensors):
+    """Every tensor that is not None is contiguous, of this type and shape, on `device`."""
+    for name, t in tensors.items():
+        if t is not None and (t.dtype != dtype or t.device != device or tuple(t.shape) != shape
+                              or not t.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous {dtype} of shape {shape} on {device}, "
+                             f"got {tuple(t.shape)} of {t.dtype} on {t.device}")
+
+
+class _on:
+    """The device of a call's tensors is current while the call is made."""
+
+    __slots__ = ("guard",)
+
+    def __init__(self, device):
+        import torch
+
+        if device.type != "cuda":
+            raise ValueError(f"tensors must be on a CUDA device, got {device}")
+        same = device.index == torch.cuda.current_device()
+        self.guard = None if same else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def op_qk_norm_rope(q, k, gamma_q=None, gamma_k=None, cos=None, sin=None, pos=None, pairs=(), eps=1e-6, q_out=None,
+                    k_out=None, stream=None):
+    """q [seqs, tokens, q_heads, dim_head], k [seqs, tokens, kv_heads, dim_head] -> both normed over each head
+    (x / sqrt(mean x^2 + eps) * gamma) and rotated: pairs[a] pairs (2i, 2i+1) turn by row pos[s, t, a] of the tables
+    cos, sin [rows, dim_head / 2].  pos int32 [seqs, tokens, len(pairs)].  q, k may be strided views (last axis
+    contiguous); q_out / k_out may be q / k themselves."""
+    import torch
+
+    S, N, H, D = q.shape
+    dev, dt = q.device, q.dtype
+    q_out = torch.empty((S, N, H, D), dtype=dt, device=dev) if q_out is None else q_out
+    k_out = torch.empty(k.shape, dtype=dt, device=dev) if k_out is None else k_out
+    _need_rows(dev, dt, q=q, k=k, q_out=q_out, k_out=k_out)
+    _need(k.shape[0] == S and k.shape[1] == N and k.shape[3] == D, "q and k must have the same seqs, tokens, dim_head")
+    _need(q_out.shape == q.shape and k_out.shape == k.shape, "outputs must have the shapes of q and k")
+    _need_flat(dev, torch.float32, (D,), gamma_q=gamma_q, gamma_k=gamma_k)
+    axes, rows = len(pairs), 0
+    if axes:
+        _need(cos is not None and sin is not None and pos is not None, "cos, sin and pos are needed with pairs")
+        rows = cos.shape[0]
+        _need_flat(dev, torch.float32, (rows, D // 2), cos=cos, sin=sin)
+        _need_flat(dev, torch.int32, (S, N, axes), pos=pos)
+    with _on(dev):
+        _check(lib().mbr_op_qk_norm_rope(
+            _view(q), _view(k), _view(q_out), _view(k_out), S, N, H, k.shape[2], D, _opt(gamma_q), _opt(gamma_k), eps,
+            _opt(cos), _opt(sin), rows, _opt(pos), axes, struct.pack(f"@{axes}i", *pairs), _dt(q), _stream(stream)))
+    return q_out, k_out
+
+
+def _opt(t):
+    return None if t is None else t.data_ptr()
+
+
+def _span(n) -> int:
+    """A window limit as the ABI takes it: 2^30 or more is none."""
+    return int(n) if n < (1 << 30) else -1
+
+
+class KVCache:
+    """A rolling key/value cache over caller-owned tensors (mbr_kv_cache).
+
+    k, v [seqs, kv_heads, slots, dim_head], or uint8 [seqs, kv_heads, slots, dim_head / 2] of 4-bit codes with k_scale,
+    v_scale [seqs, kv_heads, slots, dim_head / 32, 2] (step and offset of each 32 channels).  The first `sinks`
+    positions keep their slots, the other slots are a ring."""
+
+    __slots__ = ("k", "v", "k_scale", "v_scale", "sinks", "ring", "dtype", "device", "seqs", "kv_heads", "dim_head",
+                 "bits", "desc")
+
+    def __init__(self, k, v, k_scale=None, v_scale=None, sinks=0):
+        import torch
+
+        self.bits = 4 if k.dtype == torch.uint8 else 0
+        _need(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype and k.device == v.device,
+              "k and v must be [seqs, kv_heads, slots, ...] of the same shape, type and device")
+        _need((k_scale is not None and v_scale is not None) == (self.bits == 4),
+              "k_scale and v_scale go with 4-bit (uint8) k and v")
+        _need(k.is_contiguous() and v.is_contiguous(), "k and v must be contiguous")
+        self.seqs, self.kv_heads, slots, width = k.shape
+        self.dim_head = 2 * width if self.bits else width
+        self.dtype, self.device = (k_scale.dtype if self.bits else k.dtype), k.device
+        if self.bits:
+            _need_flat(self.device, self.dtype, (self.seqs, self.kv_heads, slots, self.dim_head // 32, 2),
+                       k_scale=k_scale, v_scale=v_scale)
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.sinks, self.ring = int(sinks), slots - int(sinks)
+        _need(self.sinks >= 0 and self.ring >= 1, "a cache needs slots beyond its sinks")
+        self.desc = _CACHE.pack(k.data_ptr(), v.data_ptr(), _opt(k_scale) or 0, _opt(v_scale) or 0, self.seqs,
+                                self.kv_heads, self.dim_head, self.sinks, self.ring, _code(self.dtype), self.bits)
+
+    @classmethod
+    def empty(cls, seqs, kv_heads, slots, dim_head, dtype, sinks=0, bits=0, device="cuda"):
+        """A cache with its own tensors (zeros): `slots` positions, `sinks` of them the first ones."""
+        import torch
+
+        if not bits:
+            k, v = (torch.zeros((seqs, kv_heads, slots, dim_head), dtype=dtype, device=device) for _ in range(2))
+            return cls(k, v, sinks=sinks)
+        _need(bits == 4, "bits must be 0 or 4")
+        k, v = (torch.zeros((seqs, kv_heads, slots, dim_head // 2), dtype=torch.uint8, device=device)
+                for _ in range(2))
+        ks, vs = (torch.zeros((seqs, kv_heads, slots, dim_head // 32, 2), dtype=dtype, device=device)
+                  for _ in range(2))
+        return cls(k, v, ks, vs, sinks=sinks)
+
+
+def _code(dtype) -> int:
+    import torch
+
+    codes = {torch.float32: FP32, torch.float16: FP16, torch.bfloat16: BF16}
+    _need(dtype in codes, f"dtype must be float32, float16 or bfloat16, got {dtype}")
+    return codes[dtype]
+
+
+def op_cache_append(cache, k, v, pos, count=None, stream=None):
+    """Writes tokens pos[s] + i, i < count[s] (None: all), of k, v [seqs, tokens, kv_heads, dim_head] into the cache;
+    pos, count int32 [seqs]."""
+    import torch
+
+    _need_rows(cache.device, cache.dtype, k=k, v=v)
+    S, N, G, D = k.shape
+    _need(v.shape == k.shape and S == cache.seqs and G == cache.kv_heads and D == cache.dim_head,
+          "k and v must be [seqs, tokens, kv_heads, dim_head] of the cache")
+    _need(pos is not None, "pos is needed")
+    _need_flat(cache.device, torch.int32, (S,), pos=pos, count=count)
+    with _on(cache.device):
+        _check(lib().mbr_op_cache_append(cache.desc, _view(k), _view(v), pos.data_ptr(), _opt(count), N,
+                                         _stream(stream)))
+
+
+def op_cache_read(cache, pos, tokens, count=None, k=None, v=None, stream=None):
+    """Values of positions pos[s] + i, i < count[s] (None: tokens), the last of them being the newest of sequence s,
+    as k, v [seqs, tokens, kv_heads, dim_head]; zeros where the cache holds nothing any more."""
+    import torch
+
+    shape = (cache.seqs, int(tokens), cache.kv_heads, cache.dim_head)
+    k = torch.empty(shape, dtype=cache.dtype, device=cache.device) if k is None else k
+    v = torch.empty(shape, dtype=cache.dtype, device=cache.device) if v is None else v
+    _need_rows(cache.device, cache.dtype, k=k, v=v)
+    _need(tuple(k.shape) == shape and tuple(v.shape) == shape, f"k and v must be {shape}")
+    _need(pos is not None, "pos is needed")
+    _need_flat(cache.device, torch.int32, (cache.seqs,), pos=pos, count=count)
+    with _on(cache.device):
+        _check(lib().mbr_op_cache_read(cache.desc, pos.data_ptr(), _opt(count), shape[1], _view(k), _view(v),
+                                       _stream(stream)))
+    return k, v
+
+
+def op_window_attention(q, k, v, left=-1, right=-1, sinks=0, scale=0.0, q_len=None, kv_len=None, gates=None, out=None,
+                        stream=None):
+    """softmax(scale q k^T) v of each query over the keys from `left` before to `right` after its position (-1: no
+    limit) and the first `sinks`, times gates [seqs, q_tokens, q_heads] if given.  q [seqs, q_tokens, q_heads,
+    dim_head], k, v [seqs, kv_tokens, kv_heads, dim_head] (views allowed); q_len, kv_len int32 [seqs]: the queries are
+    the last q_len[s] of the kv_len[s] tokens of sequence s.  -> [seqs, q_tokens, q_heads, dim_head]."""
+    import torch
+
+    S, N, H, D = q.shape
+    dev, dt = q.device, q.dtype
+    out = torch.empty((S, N, H, D), dtype=dt, device=dev) if out is None else out
+    _need_rows(dev, dt, q=q, k=k, v=v, out=out)
+    M, G = k.shape[1], k.shape[2]
+    _need(k.shape == v.shape and k.shape[0] == S and k.shape[3] == D, "k and v must be [seqs, kv_tokens, kv_heads, D]")
+    _need(out.shape == q.shape, "out must have the shape of q")
+    _need_flat(dev, torch.int32, (S,), q_len=q_len, kv_len=kv_len)
+    _need_flat(dev, torch.float32, (S, N, H), gates=gates)
+    with _on(dev):
+        _check(lib().mbr_op_window_attention(
+            _view(q), _view(k), _view(v), _view(out), S, N, M, H, G, D, _opt(q_len), _opt(kv_len), _span(left),
+            _span(right), min(int(sinks), 1 << 30), scale, _opt(gates), _dt(q), _stream(stream)))
+    return out
+
+
+def op_cache_attention(q, cache, length, left=-1, right=0, scale=0.0, gates=None, out=None, stream=None):
+    """The attention of op_window_attention for the newest tokens over a cache that holds them: q [seqs, tokens,
+    q_heads, dim_head], length int32 [seqs] tokens appended so far (these included); the cache's sinks stay visible."""
+    import torch
+
+    S, N, H, D = q.shape
+    dev = cache.device
+    out = torch.empty((S, N, H, D), dtype=q.dtype, device=dev) if out is None else out
+    _need_rows(dev, cache.dtype, q=q, out=out)
+    _need(S == cache.seqs and D == cache.dim_head, "q must be [seqs, tokens, q_heads, dim_head] of the cache")
+    _need(out.shape == q.shape, "out must have the shape of q")
+    _need(length is not None, "length is needed")
+    _need_flat(dev, torch.int32, (S,), length=length)
+    _need_flat(dev, torch.float32, (S, N, H), gates=gates)
+    with _on(dev):
+        _check(lib().mbr_op_cache_attention(_view(q), cache.desc, _view(out), length.data_ptr(), N, H, _span(left),
+                                            _span(right), scale, _opt(gates), _stream(stream)))
     return out
 
 
