@@ -304,7 +304,8 @@ MBR_API int mbr_op_attention(const void* d_q, const void* d_k, const void* d_v, 
  * All of these enqueue on `stream` and return without synchronising, allocate
  * no device memory and may be captured into a CUDA graph (call the attention
  * once before the capture: its first call on a device allocates one host-mapped
- * word).  Calls on different streams are independent.  The device that is
+ * word).  Calls on different streams are independent, each with a workspace
+ * (16-byte aligned device memory, contents free) of its own.  The device that is
  * current at the call must own the buffers and the stream.  Tokens, heads or
  * sequences of zero make a call that does nothing. */
 
@@ -388,7 +389,11 @@ MBR_API int mbr_op_window_attention(const mbr_view* q, const mbr_view* k, const 
                                     int64_t seqs, int64_t q_tokens, int64_t kv_tokens, int q_heads, int kv_heads,
                                     int dim_head, const int32_t* d_q_len, const int32_t* d_kv_len, int left,
                                     int right, int sinks, float scale, const float* d_gates, int dtype,
-                                    void* stream);
+                                    void* d_workspace, int64_t workspace_bytes, void* stream);
+/* Bytes of workspace such a call needs (0: none); host arithmetic only. */
+MBR_API int mbr_op_window_attention_workspace(int64_t seqs, int64_t q_tokens, int64_t kv_tokens, int q_heads,
+                                              int kv_heads, int dim_head, int left, int right, int sinks, int dtype,
+                                              int64_t* bytes);
 
 /* The same attention for the newest `tokens` tokens over a cache that holds
  * them already: d_length[s] tokens have been appended to sequence s, query i
@@ -399,7 +404,11 @@ MBR_API int mbr_op_window_attention(const mbr_view* q, const mbr_view* k, const 
  * [seqs][tokens][q_heads] fp32 or null. */
 MBR_API int mbr_op_cache_attention(const mbr_view* q, const mbr_kv_cache* cache, const mbr_view* out,
                                    const int32_t* d_length, int64_t tokens, int q_heads, int left, int right,
-                                   float scale, const float* d_gates, void* stream);
+                                   float scale, const float* d_gates, void* d_workspace, int64_t workspace_bytes,
+                                   void* stream);
+/* Bytes of workspace such a call needs (0: none); host arithmetic only. */
+MBR_API int mbr_op_cache_attention_workspace(const mbr_kv_cache* cache, int64_t tokens, int q_heads, int left,
+                                             int right, int64_t* bytes);
 
 /* Host tables of MelBandRoformer::compute_rotary_cos_sin
  * (src/model_mel_band_roformer.cu:270-300): h_cos, h_sin [L][dim_head/2]. */

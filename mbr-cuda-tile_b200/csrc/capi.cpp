@@ -624,21 +624,41 @@ MBR_API int mbr_op_window_attention(const mbr_view* q, const mbr_view* k, const 
                                     int64_t seqs, int64_t q_tokens, int64_t kv_tokens, int q_heads, int kv_heads,
                                     int dim_head, const int32_t* d_q_len, const int32_t* d_kv_len, int left,
                                     int right, int sinks, float scale, const float* d_gates, int dtype,
-                                    void* stream) {
+                                    void* d_workspace, int64_t workspace_bytes, void* stream) {
     return guard([&] {
         mbr::streamops::window_attention(view_or_empty(q), view_or_empty(k), view_or_empty(v), view_or_empty(out),
                                          seqs, q_tokens, kv_tokens, q_heads, kv_heads, dim_head, d_q_len, d_kv_len,
-                                         left, right, sinks, scale, d_gates, dtype, (cudaStream_t)stream);
+                                         left, right, sinks, scale, d_gates, dtype, d_workspace, workspace_bytes,
+                                         (cudaStream_t)stream);
     });
 }
 
 MBR_API int mbr_op_cache_attention(const mbr_view* q, const mbr_kv_cache* cache, const mbr_view* out,
                                    const int32_t* d_length, int64_t tokens, int q_heads, int left, int right,
-                                   float scale, const float* d_gates, void* stream) {
+                                   float scale, const float* d_gates, void* d_workspace, int64_t workspace_bytes,
+                                   void* stream) {
     return guard([&] {
         need(cache, "null argument");
         mbr::streamops::cache_attention(view_or_empty(q), *cache, view_or_empty(out), d_length, tokens, q_heads, left,
-                                        right, scale, d_gates, (cudaStream_t)stream);
+                                        right, scale, d_gates, d_workspace, workspace_bytes, (cudaStream_t)stream);
+    });
+}
+
+MBR_API int mbr_op_window_attention_workspace(int64_t seqs, int64_t q_tokens, int64_t kv_tokens, int q_heads,
+                                              int kv_heads, int dim_head, int left, int right, int sinks, int dtype,
+                                              int64_t* bytes) {
+    return guard([&] {
+        need(bytes, "null argument");
+        *bytes = mbr::streamops::window_attention_workspace(seqs, q_tokens, kv_tokens, q_heads, kv_heads, dim_head,
+                                                            left, right, sinks, dtype);
+    });
+}
+
+MBR_API int mbr_op_cache_attention_workspace(const mbr_kv_cache* cache, int64_t tokens, int q_heads, int left,
+                                             int right, int64_t* bytes) {
+    return guard([&] {
+        need(cache && bytes, "null argument");
+        *bytes = mbr::streamops::cache_attention_workspace(*cache, tokens, q_heads, left, right);
     });
 }
 

@@ -9,23 +9,29 @@
 namespace mbr {
 namespace streamops {
 
-bool check_cache(const mbr_kv_cache& c) {
+void check_cache_fields(const mbr_kv_cache& c) {
     MBR_CHECK(c.seqs >= 0 && c.kv_heads >= 0 && c.sinks >= 0, "kv cache: negative size");
     MBR_CHECK(c.ring >= 1 && c.sinks < (1 << 30) && c.ring < (1 << 30), "kv cache: ring must be 1..2^30 - 1");
     MBR_CHECK(c.dtype == DT_F32 || c.dtype == DT_F16 || c.dtype == DT_BF16, "kv cache: dtype must be fp32, fp16 or bf16");
     MBR_CHECK(c.bits == 0 || c.bits == 4, "kv cache: bits must be 0 or 4");
     MBR_CHECK(c.dim_head >= 8 && c.dim_head <= 128 && c.dim_head % 8 == 0,
               "kv cache: dim_head must be a multiple of 8 up to 128");
+    MBR_CHECK(c.bits == 0 || (c.dtype != DT_F32 && c.dim_head % kGroup == 0),
+              "kv cache: 4 bits need fp16 or bf16 and dim_head a multiple of 32");
+    MBR_CHECK(c.seqs == 0 || c.kv_heads == 0 ||
+                  c.seqs <= ((int64_t)1 << 40) / c.kv_heads / ((int64_t)c.sinks + c.ring),
+              "kv cache: too large");
+}
+
+bool check_cache(const mbr_kv_cache& c) {
+    check_cache_fields(c);
     const bool some = c.seqs > 0 && c.kv_heads > 0;
     MBR_CHECK(!some || (c.k && c.v), "kv cache: null buffer");
     MBR_CHECK((((uintptr_t)c.k | (uintptr_t)c.v) & 15) == 0, "kv cache: buffers must be 16-byte aligned");
     if (c.bits == 4) {
-        MBR_CHECK(c.dtype != DT_F32 && c.dim_head % kGroup == 0,
-                  "kv cache: 4 bits need fp16 or bf16 and dim_head a multiple of 32");
         MBR_CHECK(!some || (c.k_scale && c.v_scale), "kv cache: 4 bits need the steps and offsets");
         MBR_CHECK((((uintptr_t)c.k_scale | (uintptr_t)c.v_scale) & 15) == 0, "kv cache: buffers must be 16-byte aligned");
     }
-    MBR_CHECK(!some || c.seqs <= ((int64_t)1 << 40) / c.kv_heads / ((int64_t)c.sinks + c.ring), "kv cache: too large");
     return c.bits == 4;
 }
 

@@ -25,11 +25,25 @@ void cache_read(const mbr_kv_cache& c, const int32_t* pos, const int32_t* count,
 
 void window_attention(const mbr_view& q, const mbr_view& k, const mbr_view& v, const mbr_view& out, int64_t seqs,
                       int64_t Nq, int64_t Nk, int Hq, int Hkv, int D, const int32_t* q_len, const int32_t* kv_len,
-                      int left, int right, int sinks, float scale, const float* gates, int dtype, cudaStream_t st);
+                      int left, int right, int sinks, float scale, const float* gates, int dtype, void* workspace,
+                      int64_t workspace_bytes, cudaStream_t st);
+int64_t window_attention_workspace(int64_t seqs, int64_t Nq, int64_t Nk, int Hq, int Hkv, int D, int left, int right,
+                                   int sinks, int dtype);
 void cache_attention(const mbr_view& q, const mbr_kv_cache& c, const mbr_view& out, const int32_t* length,
-                     int64_t tokens, int Hq, int left, int right, float scale, const float* gates, cudaStream_t st);
+                     int64_t tokens, int Hq, int left, int right, float scale, const float* gates, void* workspace,
+                     int64_t workspace_bytes, cudaStream_t st);
+int64_t cache_attention_workspace(const mbr_kv_cache& c, int64_t tokens, int Hq, int left, int right);
 
-// Checks a cache's fields (throws); true when its rows are 4-bit codes.
+// Current device (checked against the per-device tables below).
+constexpr int kMaxStreamDevices = 64;
+int stream_device();
+// Error word that the attention kernels' bounded waits set: host memory that
+// the device writes, so the host sees it without a copy.  Throws if it is set
+// (and clears it): the call before ran out of a wait.
+int* stream_error_word();
+
+// Checks a cache's sizes and type; check_cache its buffers too (true when its rows are 4-bit codes).
+void check_cache_fields(const mbr_kv_cache& c);
 bool check_cache(const mbr_kv_cache& c);
 // True if every row of the view starts on a 16-byte boundary (es: element size).
 inline bool rows_aligned16(const mbr_view& v, int es) {

@@ -32,7 +32,7 @@ EXPORTS = [
     "mbr_sync_check", "mbr_profile_enable", "mbr_profile_read",
     "mbr_op_rms_norm", "mbr_op_add", "mbr_op_gelu", "mbr_op_sigmoid_gate", "mbr_op_rope", "mbr_op_attention", "mbr_op_linear", "mbr_op_ffn",
     "mbr_op_qk_norm_rope", "mbr_op_cache_append", "mbr_op_cache_read", "mbr_op_window_attention",
-    "mbr_op_cache_attention",
+    "mbr_op_cache_attention", "mbr_op_window_attention_workspace", "mbr_op_cache_attention_workspace",
     "mbr_rope_tables",
     "mbr_op_band_gather", "mbr_op_mask_scatter", "mbr_op_stft", "mbr_op_istft", "mbr_op_istft_noalloc",
     "mbr_plan_shard", "mbr_wav_info", "mbr_wav_read", "mbr_wav_write",
@@ -100,8 +100,10 @@ def lib():
         L.mbr_op_cache_append.argtypes = [vp, vp, vp, vp, vp, i64, vp]
         L.mbr_op_cache_read.argtypes = [vp, vp, vp, i64, vp, vp, vp]
         L.mbr_op_window_attention.argtypes = [vp, vp, vp, vp, i64, i64, i64, c_int, c_int, c_int, vp, vp, c_int, c_int,
-                                              c_int, c_float, fp, c_int, vp]
-        L.mbr_op_cache_attention.argtypes = [vp, vp, vp, vp, i64, c_int, c_int, c_int, c_float, fp, vp]
+                                              c_int, c_float, fp, c_int, vp, i64, vp]
+        L.mbr_op_cache_attention.argtypes = [vp, vp, vp, vp, i64, c_int, c_int, c_int, c_float, fp, vp, i64, vp]
+        L.mbr_op_window_attention_workspace.argtypes = [i64, i64, i64] + [c_int] * 7 + [i64p]
+        L.mbr_op_cache_attention_workspace.argtypes = [vp, i64, c_int, c_int, c_int, i64p]
         L.mbr_rope_tables.argtypes = [c_int, c_int, fp, fp]
         L.mbr_op_band_gather.argtypes = [vp, fp, c_int, c_int, fp, c_int, vp]
         L.mbr_op_mask_scatter.argtypes = [vp, fp, fp, c_int, c_int, c_int, fp, c_int, vp]
@@ -327,6 +329,20 @@ def _opt(t):
     return None if t is None else t.data_ptr()
 
 
+def _workspace(n, device, stream):
+    """n bytes of device memory for one call on `stream` (None: the current one); freed in that stream's order."""
+    import torch
+
+    if not n:
+        return None
+    if stream is None:
+        return torch.empty(n, dtype=torch.uint8, device=device)
+    if isinstance(stream, int):
+        stream = torch.cuda.ExternalStream(stream, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(n, dtype=torch.uint8, device=device)
+
+
 def _span(n) -> int:
     """A window limit as the ABI takes it: 2^30 or more is none."""
     return int(n) if n < (1 << 30) else -1
@@ -438,10 +454,13 @@ def op_window_attention(q, k, v, left=-1, right=-1, sinks=0, scale=0.0, q_len=No
     _need(out.shape == q.shape, "out must have the shape of q")
     _need_flat(dev, torch.int32, (S,), q_len=q_len, kv_len=kv_len)
     _need_flat(dev, torch.float32, (S, N, H), gates=gates)
+    left, right, sinks, n = _span(left), _span(right), min(int(sinks), 1 << 30), ctypes.c_int64()
+    _check(lib().mbr_op_window_attention_workspace(S, N, M, H, G, D, left, right, sinks, _dt(q), ctypes.byref(n)))
     with _on(dev):
+        work = _workspace(n.value, dev, stream)
         _check(lib().mbr_op_window_attention(
-            _view(q), _view(k), _view(v), _view(out), S, N, M, H, G, D, _opt(q_len), _opt(kv_len), _span(left),
-            _span(right), min(int(sinks), 1 << 30), scale, _opt(gates), _dt(q), _stream(stream)))
+            _view(q), _view(k), _view(v), _view(out), S, N, M, H, G, D, _opt(q_len), _opt(kv_len), left, right, sinks,
+            scale, _opt(gates), _dt(q), _opt(work), n.value, _stream(stream)))
     return out
 
 
@@ -459,9 +478,12 @@ def op_cache_attention(q, cache, length, left=-1, right=0, scale=0.0, gates=None
     _need(length is not None, "length is needed")
     _need_flat(dev, torch.int32, (S,), length=length)
     _need_flat(dev, torch.float32, (S, N, H), gates=gates)
+    left, right, n = _span(left), _span(right), ctypes.c_int64()
+    _check(lib().mbr_op_cache_attention_workspace(cache.desc, N, H, left, right, ctypes.byref(n)))
     with _on(dev):
-        _check(lib().mbr_op_cache_attention(_view(q), cache.desc, _view(out), length.data_ptr(), N, H, _span(left),
-                                            _span(right), scale, _opt(gates), _stream(stream)))
+        work = _workspace(n.value, dev, stream)
+        _check(lib().mbr_op_cache_attention(_view(q), cache.desc, _view(out), length.data_ptr(), N, H, left, right, scale,
+                                            _opt(gates), _opt(work), n.value, _stream(stream)))
     return out
 
 

@@ -64,7 +64,7 @@ def test_entry_points_refuse_without_a_gpu():
 
     def window(Hq=1, Hkv=1, D=64, N=1, M=1, sinks=0, dtype=1, scale=0.0, q=view):
         return L.mbr_op_window_attention(q, view, view, view, 1, N, M, Hq, Hkv, D, None, None, -1, -1, sinks, scale, None,
-                                         dtype, None)
+                                         dtype, None, 0, None)
 
     def cache(dtype=1, bits=0, D=64, ring=4, sinks=0, k=4096):
         return cudasep._CACHE.pack(k, k, k if bits else 0, k if bits else 0, 1, 1, D, sinks, ring, dtype, bits)
@@ -78,8 +78,9 @@ def test_entry_points_refuse_without_a_gpu():
                window(q=None), append(None), append(cache(dtype=2)), append(cache(bits=3)), append(cache(dtype=0, bits=4)),
                append(cache(bits=4, D=40)), append(cache(ring=0)), append(cache(sinks=-1)), append(cache(D=4)),
                append(cache(k=4104)), append(cache(), tokens=-1), append(cache(), pos=None),
-               L.mbr_op_cache_attention(view, cache(), view, None, 1, 1, -1, 0, 0.0, None, None),
-               L.mbr_op_cache_attention(view, None, view, one, 1, 1, -1, 0, 0.0, None, None)]
+               L.mbr_op_cache_attention(view, cache(), view, None, 1, 1, -1, 0, 0.0, None, None, 0, None),
+               L.mbr_op_cache_attention(view, cache(), view, one, 1, 1, -1, 0, 0.0, None, None, 0, None),
+               L.mbr_op_cache_attention(view, None, view, one, 1, 1, -1, 0, 0.0, None, None, 0, None)]
     assert refused == [1] * len(refused)
     assert L.mbr_last_error()
     # nothing to do is no error, and needs no buffers
