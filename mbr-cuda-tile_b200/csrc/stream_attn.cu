@@ -84,6 +84,7 @@ AttnArgs common_args(const mbr_view& q, const mbr_view& out, int64_t seqs, int64
     a.q_seq = q.seq, a.q_tok = q.token, a.q_head = q.head;
     a.o_seq = out.seq, a.o_tok = out.token, a.o_head = out.head;
     a.seqs = seqs, a.Nq = (int)Nq, a.Hq = Hq, a.Hkv = Hkv, a.D = D, a.G = Hkv ? Hq / Hkv : 1;
+    a.by_G = FastDiv((unsigned)std::max(1, a.G)), a.by_Hkv = FastDiv((unsigned)std::max(1, Hkv));
     a.left = limit(left), a.right = limit(right), a.sinks = sinks;
     a.scale = scale == 0.f ? 1.f / std::sqrt((float)D) : scale;
     a.gates = gates;
@@ -136,7 +137,7 @@ void window_attention(const mbr_view& q, const mbr_view& k, const mbr_view& v, c
     a.q_len = q_len, a.kv_len = kv_len;
     if (few_rows(a) && step_supported(a, dtype, false)) {
         const StepPlan pl = plan_of(a, Nk);
-        MBR_CHECK(workspace && workspace_bytes >= pl.bytes, "window_attention: workspace too small");
+        MBR_CHECK(pl.bytes == 0 || (workspace && workspace_bytes >= pl.bytes), "window_attention: workspace too small");
         attend_step(a, dtype, false, false, pl, workspace, st);
         return;
     }
@@ -163,7 +164,7 @@ void cache_attention(const mbr_view& q, const mbr_kv_cache& c, const mbr_view& o
     a.kv_len = length;
     if (step_supported(a, c.dtype, true)) {
         const StepPlan pl = plan_of(a, a.slots);
-        MBR_CHECK(workspace && workspace_bytes >= pl.bytes, "cache_attention: workspace too small");
+        MBR_CHECK(pl.bytes == 0 || (workspace && workspace_bytes >= pl.bytes), "cache_attention: workspace too small");
         attend_step(a, c.dtype, true, q4, pl, workspace, st);
         return;
     }

@@ -6,11 +6,11 @@
 // the matrix products only have to keep out of the way.  One CTA per SM; each of
 // its warps works alone: it walks part of the keys of one (sequence, key head, row
 // tile), with a ring of its own in shared memory that it refills by bulk copies
-// (the rows of a cache are contiguous: two copies a unit of 16 or 32 keys), so
-// all the SM's shared memory is loads in flight and no warp waits for another.
-// The parts' results (fp32, with their running maximum and sum) go to a
-// workspace and a second kernel, launched to overlap this one's end, joins them
-// in a fixed order.
+// (the rows of a cache are contiguous: one copy for 32 keys, one for their
+// values), so all the SM's shared memory is loads in flight and no warp waits
+// for another.  The parts' results (fp32, with their offset and sum) are joined
+// in a fixed order: up to a CTA's warps through shared memory, more (few
+// sequences, many keys) through a workspace by a second kernel.
 // The products are 16 x 8 x 16 warp products whose operands come from the rows as
 // they lie, by free choice of the orders:
 //  - S = Q K^T contracts over channels, and the order of a contraction is
@@ -40,27 +40,51 @@ namespace {
 
 using namespace sm100;
 
-// A warp's ring: SLOTS units of UNIT keys' rows (and, 4 bits, steps and offsets).
+constexpr int UNIT = 32;  // keys a warp works on at a time
+
+// A warp's ring: SLOTS times the rows of one unit's keys or values (and, 4
+// bits, their steps and offsets).
 template <int DP, bool Q4>
 struct StepCfg {
-    static constexpr int WARPS = DP == 128 ? 8 : 16;
-    static constexpr int UNIT = Q4 || DP == 32 ? 32 : 16;
+    static constexpr int WARPS = step_warps(DP);
     static constexpr int ROW = Q4 ? DP / 2 : DP * 2;  // most bytes of a row
     static constexpr int SROW = Q4 ? DP / kGroup * 4 : 0;
-    static constexpr int SLOT = 2 * UNIT * (ROW + SROW);
+    static constexpr int SLOT = UNIT * (ROW + SROW);
     static constexpr int BUDGET = 200 * 1024 / WARPS;
-    static constexpr int SLOTS = BUDGET / SLOT < 4 ? BUDGET / SLOT : 4;
-    static_assert(SLOTS >= 3, "two units in flight while one is read");
-    static constexpr int TOTAL = WARPS * SLOTS * (SLOT + 8);
+    static constexpr int SLOTS = BUDGET / SLOT < 8 ? BUDGET / SLOT : 8;
+    static_assert(SLOTS >= 3, "two copies in flight while one is read");
+    static constexpr int RING = SLOTS * SLOT > 16 * (DP + 2) * 4 ? SLOTS * SLOT : 16 * (DP + 2) * 4;  // holds a result
+    static constexpr int TOTAL = WARPS * (RING + SLOTS * 8);
 };
 
+// Shared memory is addressed by its 32-bit addresses throughout: a unit's loads
+// are one register plus constants.
 // Untiled bulk copy of `bytes` (a multiple of 16, both addresses 16-byte
 // aligned), completion counted on `bar`.
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                     smem_u32(dst)),
-                 "l"(src), "r"(bytes), "r"(smem_u32(bar))
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "l"(src), "r"(bytes), "r"(bar)
                  : "memory");
+}
+__device__ __forceinline__ void expect_bytes(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// Waits (with a limit) for the phase of the given parity; what runs out is
+// recorded in *err and passed: the host sees the error word, the results are void.
+__device__ __forceinline__ void wait_bytes(uint32_t bar, uint32_t parity, int* err) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (!ok) mbar_wait((uint64_t*)__cvta_shared_to_generic(bar), parity, err);
+}
+template <int N>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(N) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -90,39 +114,62 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16*) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// A constant the compiler keeps in a register instead of writing it out at each use.
+__device__ __forceinline__ uint32_t held(uint32_t c) {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %1;" : "=r"(r) : "r"(c));
+    return r;
+}
+// What widening codes takes: the mask of two codes, 1024 (fp16) or 128 (bf16)
+// in both halves, whose last bits a code fits into, and minus that and eight.
+template <typename T>
+struct Widen;
+template <>
+struct Widen<__half> {
+    uint32_t mask = held(0x000f000fu), base = held(0x64006400u), less = held(0xe408e408u);  // -1032
+};
+template <>
+struct Widen<__nv_bfloat16> {
+    uint32_t mask = held(0x000f000fu), base = held(0x43004300u), less = held(0xc308c308u);  // -136
+};
 // The two values that the codes at bits 4i and 16 + 4i of x stand for: code -
 // 8 (exact in 16 bits), times the step plus the offset in one rounding.
-// sm: (step, offset) of the lower value in s.x / m.x, of the upper in s.y / m.y.
-__device__ __forceinline__ uint32_t widen(uint32_t x, int i, uint32_t s, uint32_t m, __half*) {
-    const uint32_t b = ((x >> (4 * i)) & 0x000f000fu) | 0x64006400u;  // 1024 + code
-    const __half2 u = __hadd2(*reinterpret_cast<const __half2*>(&b), __floats2half2_rn(-1032.f, -1032.f));
-    const __half2 v = __hfma2(u, *reinterpret_cast<const __half2*>(&s), *reinterpret_cast<const __half2*>(&m));
-    return *reinterpret_cast<const uint32_t*>(&v);
+// s, m: step and offset of both.
+__device__ __forceinline__ uint32_t masked(uint32_t x, uint32_t mask, uint32_t base) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "r"(mask), "r"(base));  // (x & mask) | base
+    return r;
 }
-__device__ __forceinline__ uint32_t widen(uint32_t x, int i, uint32_t s, uint32_t m, __nv_bfloat16*) {
-    const uint32_t b = ((x >> (4 * i)) & 0x000f000fu) | 0x43004300u;  // 128 + code
-    const __nv_bfloat162 u =
-        __hadd2(*reinterpret_cast<const __nv_bfloat162*>(&b), __floats2bfloat162_rn(-136.f, -136.f));
-    const __nv_bfloat162 v =
-        __hfma2(u, *reinterpret_cast<const __nv_bfloat162*>(&s), *reinterpret_cast<const __nv_bfloat162*>(&m));
-    return *reinterpret_cast<const uint32_t*>(&v);
+__device__ __forceinline__ uint32_t widen(uint32_t x, int i, uint32_t s, uint32_t m, const Widen<__half>& w) {
+    uint32_t u = masked(x >> (4 * i), w.mask, w.base), v;
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(u) : "r"(u), "r"(w.less));
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(v) : "r"(u), "r"(s), "r"(m));
+    return v;
+}
+__device__ __forceinline__ uint32_t widen(uint32_t x, int i, uint32_t s, uint32_t m, const Widen<__nv_bfloat16>& w) {
+    uint32_t u = masked(x >> (4 * i), w.mask, w.base), v;
+    asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(u) : "r"(u), "r"(w.less));
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(v) : "r"(u), "r"(s), "r"(m));
+    return v;
 }
 
+// BYTES bytes of shared memory at p (volatile: in order with the waits and copies).
 template <int BYTES>
-__device__ __forceinline__ void load_words(uint32_t* dst, const uint8_t* p) {
+__device__ __forceinline__ void load_words(uint32_t* dst, uint32_t p) {
     if constexpr (BYTES == 2) {
-        dst[0] = *reinterpret_cast<const uint16_t*>(p);
+        uint16_t h;
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(p));
+        dst[0] = h;
     } else if constexpr (BYTES == 4) {
-        dst[0] = *reinterpret_cast<const uint32_t*>(p);
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(dst[0]) : "r"(p));
     } else if constexpr (BYTES == 8) {
-        const uint2 v = *reinterpret_cast<const uint2*>(p);
-        dst[0] = v.x, dst[1] = v.y;
+        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(dst[0]), "=r"(dst[1]) : "r"(p));
     } else {
 #pragma unroll
-        for (int i = 0; i < BYTES / 16; ++i) {
-            const uint4 v = *(reinterpret_cast<const uint4*>(p) + i);
-            dst[4 * i] = v.x, dst[4 * i + 1] = v.y, dst[4 * i + 2] = v.z, dst[4 * i + 3] = v.w;
-        }
+        for (int i = 0; i < BYTES / 16; ++i)
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(dst[4 * i]), "=r"(dst[4 * i + 1]), "=r"(dst[4 * i + 2]), "=r"(dst[4 * i + 3])
+                         : "r"(p + 16 * i));
     }
 }
 
@@ -144,9 +191,9 @@ __device__ __forceinline__ TileKeys tile_keys(const AttnArgs& a, int64_t s, int 
     lengths<CACHED>(a, s, k.n, k.m);
     k.ns = k.LO = k.total = 0;
     // from the first token's lower end to the last one's upper end
-    const int i0 = r0 / a.G, i1 = min((r0 + rows - 1) / a.G, k.n - 1);
+    const int i0 = (int)a.by_G.div(r0), i1 = min((int)a.by_G.div(r0 + rows - 1), k.n - 1);
     if (i0 <= i1) {
-        const Window w0 = row_window<CACHED>(a, i0, k.n, k.m), w1 = row_window<CACHED>(a, i1, k.n, k.m);
+        const Window w0 = row_window<CACHED>(a, i0, k.n, k.m), w1 = i1 == i0 ? w0 : row_window<CACHED>(a, i1, k.n, k.m);
         k.ns = min(a.sinks, w1.hi);
         k.LO = max(CACHED ? max(w0.lo, k.m - a.ring) : w0.lo, k.ns);
         k.total = k.ns + max(w1.hi - k.LO, 0);
@@ -155,8 +202,9 @@ __device__ __forceinline__ TileKeys tile_keys(const AttnArgs& a, int64_t s, int 
 }
 template <bool CACHED>
 __device__ __forceinline__ RowKeys row_keys(const AttnArgs& a, const TileKeys& k, int r0, int r, int rows) {
+    if (a.Nq == 1) return RowKeys{r < rows ? k.ns : 0, r < rows ? k.ns : 0, r < rows ? k.total : 0};
     RowKeys w{0, 0, 0};
-    const int i = (r0 + r) / a.G;
+    const int i = (int)a.by_G.div(r0 + r);
     if (r < rows && i < k.n) {
         const Window x = row_window<CACHED>(a, i, k.n, k.m);
         if (x.hi > x.lo || x.first > 0) {
@@ -168,45 +216,81 @@ __device__ __forceinline__ RowKeys row_keys(const AttnArgs& a, const TileKeys& k
     return w;
 }
 
+// Row r of a tile from its sums v (channels lane, lane + 32, ...) and l: divided,
+// gated, rounded and written, by one warp.
+template <typename T, int DP, bool Q4, bool CACHED>
+__device__ __forceinline__ void finish_row(const AttnArgs& a, const TileKeys& tk, const RowKeys& k, int64_t s, int hk,
+                                           int rr, float (&v)[DP / 32], float l) {
+    const int lane = threadIdx.x & 31, i = (int)a.by_G.div(rr), h = hk * a.G + rr - i * a.G;
+    const float gate = a.gates ? __ldg(a.gates + (s * a.Nq + i) * a.Hq + h) : 1.f;
+    const bool sees = k.f > 0 || k.b > k.a;
+    const float inv = sees ? gate / l : 0.f;
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < DP / 32; ++e) {
+        v[e] = sees ? v[e] * inv : 0.f;
+        bad |= lane + 32 * e < a.D && !isfinite(v[e]);
+    }
+    if (__any_sync(0xffffffffu, bad)) {
+        attend_row<T, CACHED, Q4>(a, s, i, h, tk.n, tk.m);
+    } else {
+        T* out = (T*)a.out + s * a.o_seq + (int64_t)i * a.o_tok + (int64_t)h * a.o_head;
+#pragma unroll
+        for (int e = 0; e < DP / 32; ++e)
+            if (lane + 32 * e < a.D) out[lane + 32 * e] = from_f32<T>(v[e]);
+    }
+}
+// Factor that brings sums with offset m to offset top.
+__device__ __forceinline__ float to_offset(float m, float top) { return m == -INFINITY ? 0.f : ex2_approx(m - top); }
+
 // HALF: at most 8 rows; EX: the head size is DP itself.
 template <typename T, int DP, bool Q4, bool CACHED, bool HALF, bool EX>
 __global__ void __launch_bounds__(StepCfg<DP, Q4>::WARPS * 32, 1) attend_step_kernel(const StepArgs p) {
     constexpr int KS = DP / 16;  // contraction steps of S
     constexpr int NT = DP / 8;   // channel tiles of O
     using Cfg = StepCfg<DP, Q4>;
-    constexpr int ROWS = HALF ? 8 : 16, UNIT = Cfg::UNIT, SLOTS = Cfg::SLOTS, JT = UNIT / 8;
+    constexpr int ROWS = HALF ? 8 : 16, SLOTS = Cfg::SLOTS, JT = UNIT / 8;
     extern __shared__ __align__(128) uint8_t smem[];
     const AttnArgs& a = p.a;
     const int D = EX ? DP : a.D;
     const int rb = Q4 ? D / 2 : D * 2, sb = Q4 ? D / kGroup * 4 : 0;  // bytes of a row, of its steps and offsets
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    uint8_t* const ring = smem + warp * (SLOTS * Cfg::SLOT);
-    uint64_t* const bar = reinterpret_cast<uint64_t*>(smem + Cfg::WARPS * SLOTS * Cfg::SLOT) + warp * SLOTS;
+    const uint32_t ring = smem_u32(smem) + warp * Cfg::RING;
+    const uint32_t bar = smem_u32(smem) + Cfg::WARPS * Cfg::RING + warp * (SLOTS * 8);
     if (lane < SLOTS) {
-        mbar_init(&bar[lane], 1);
+        mbar_init(reinterpret_cast<uint64_t*>(smem + Cfg::WARPS * Cfg::RING) + warp * SLOTS + lane, 1);
         fence_barrier_init();
     }
     __syncwarp();
     // the join kernel may be scheduled as this grid's CTAs end (it waits for all of them)
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    uint32_t use = 0;  // units fetched so far by this warp: slot and parity
+    if (p.outer > 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    int st = 0;           // slot to be read next
+    uint32_t parity = 0;  // and the parity of its use
+    auto after = [](int x, int n) { return x + n >= SLOTS ? x + n - SLOTS : x + n; };
     const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;  // a negative scale turns Q's signs
     const float scale = fabsf(p.scale_log2);
+    const Widen<T> wd;
 
-    const int64_t segs = p.items * p.parts;
-    // neighbouring parts go to different SMs: what lies unevenly is spread
-    for (int64_t seg = (int64_t)warp * gridDim.x + blockIdx.x; seg < segs; seg += (int64_t)gridDim.x * Cfg::WARPS) {
-        const int64_t item = seg / p.parts;
-        const int part = (int)(seg - item * p.parts);
-        const int64_t hs = item / p.tiles;
+    // Neighbouring shares go to different SMs: what lies unevenly is spread.
+    const int inner = 1 << p.inner_log2, group = warp >> p.inner_log2, part = warp & (inner - 1);
+    const unsigned todo = p.items * p.outer, stride = gridDim.x * (Cfg::WARPS >> p.inner_log2);
+    for (unsigned seg = group * gridDim.x + blockIdx.x; seg < todo; seg += stride) {
+        const unsigned item = p.by_outer.div(seg), share = seg - item * p.outer;
+        const unsigned hs = p.by_tiles.div(item);
         const int r0 = (int)(item - hs * p.tiles) * ROWS;
-        const int64_t s = hs / a.Hkv;
-        const int hk = (int)(hs - s * a.Hkv);
+        const unsigned sq = a.by_Hkv.div(hs);
+        const int64_t s = sq;
+        const int hk = (int)(hs - sq * a.Hkv);
         const int rows = min(ROWS, a.Nq * a.G - r0);
         const TileKeys tk = tile_keys<CACHED>(a, s, r0, rows);
         const int total = tk.total, ns = tk.ns;
         const int units = (total + UNIT - 1) / UNIT;
-        const int c0 = (int)((int64_t)units * part / p.parts), c1 = (int)((int64_t)units * (part + 1) / p.parts);
+        // this CTA's units (units / outer, the first units % outer shares one more), of which the group's warps
+        // take every inner-th: they read neighbouring rows at about the same time
+        const int each = (int)p.by_outer.div(units), more = units - each * p.outer;
+        const int c0 = each * (int)share + min((int)share, more) + part,
+                  c1 = each * (int)(share + 1) + min((int)share + 1, more);
+        const int mine = c1 > c0 ? (c1 - c0 + inner - 1) >> p.inner_log2 : 0;
 
         // slot of key index u; a ring starts over at most once (total - ns <= ring), at index `wrap`
         const unsigned ring0 =
@@ -215,51 +299,73 @@ __global__ void __launch_bounds__(StepCfg<DP, Q4>::WARPS * 32, 1) attend_step_ke
         auto slot = [&](int u) -> int64_t { return u < ns ? u : (int64_t)ring0 + (u - ns) - (u >= wrap ? a.ring : 0); };
         const uint8_t* kb0 = (const uint8_t*)a.k + s * p.k_seq + hk * p.k_head;
         const uint8_t* vb0 = (const uint8_t*)a.v + s * p.v_seq + hk * p.v_head;
-        auto fetch = [&](int c, uint32_t n) {  // unit c (none past the end) into the n-th use of the ring
-            if (c < c1) {
-                uint8_t* dk = ring + (n % SLOTS) * Cfg::SLOT;
-                uint8_t* dv = dk + UNIT * Cfg::ROW;
-                const int u0 = c * UNIT, u1 = min(u0 + UNIT, total);
-                if (p.packed) {
-                    if (lane == 0) {  // whole runs of rows: the first tokens, up to the ring's end, from its start
-                        uint64_t* b = &bar[n % SLOTS];
-                        mbar_arrive_expect_tx(b, (uint32_t)(2 * (u1 - u0) * rb));
-                        for (int u = u0; u < u1;) {
-                            const int to = min(u1, u < ns ? ns : u < wrap ? wrap : total);
-                            const int64_t src = slot(u) * rb;
-                            const uint32_t at = (uint32_t)((u - u0) * rb), bytes = (uint32_t)((to - u) * rb);
-                            bulk_load(dk + at, kb0 + src, bytes, b);
-                            bulk_load(dv + at, vb0 + src, bytes, b);
-                            u = to;
+        // the n-th copy of this part (unit n / 2: keys, then values; none past the end) into a slot of the ring
+        const int copies = 2 * mine;
+        const int64_t s0 = s * p.s_seq + hk * p.s_head;
+        // units [run_lo, run_hi) lie whole in one run of cache rows; unit c's keys start at run_k + c * UNIT * rb
+        int run_lo = 0, run_hi = 0;
+        const uint8_t *run_k = nullptr, *run_v = nullptr;
+        auto fetch = [&](int n, int to_slot) {
+            if (n < copies) {
+                const uint32_t dst = ring + to_slot * Cfg::SLOT;
+                const int c = c0 + ((n >> 1) << p.inner_log2);
+                if constexpr (CACHED) {
+                    if (lane == 0) {
+                        const uint32_t b = bar + to_slot * 8;
+                        if (c >= run_lo && c < run_hi) {
+                            expect_bytes(b, UNIT * rb);
+                            bulk_load(dst, (n & 1 ? run_v : run_k) + (int64_t)c * (UNIT * rb), UNIT * rb, b);
+                        } else {  // the first tokens, the ring's end, its start, the last unit: run by run
+                            const int u0 = c * UNIT, u1 = min(u0 + UNIT, total);
+                            expect_bytes(b, (uint32_t)((u1 - u0) * rb));
+                            int to = 0;
+                            for (int u = u0; u < u1; u = to) {
+                                const int end = u < ns ? ns : u < wrap ? wrap : total;
+                                to = min(u1, end);
+                                const int64_t at = slot(u);
+                                bulk_load(dst + (u - u0) * rb, (n & 1 ? vb0 : kb0) + at * rb, (uint32_t)((to - u) * rb), b);
+                                // the run that this unit ends in
+                                run_lo = c + 1, run_hi = end / UNIT;
+                                run_k = kb0 + (at - u) * rb, run_v = vb0 + (at - u) * rb;
+                            }
                         }
                     }
                 } else {  // rows apart: 16-byte copies, neighbouring lanes on one row
-                    const int per = rb >> 4;
+                    const int per = rb >> 4, u0 = c * UNIT, u1 = min(u0 + UNIT, total);
+                    const int64_t tok = n & 1 ? p.v_tok : p.k_tok;
+                    const uint8_t* src = n & 1 ? vb0 : kb0;
                     for (int j = lane; j < (u1 - u0) * per; j += 32) {
                         const int r = j / per, o = (j - r * per) * 16;
-                        const int64_t sl = slot(u0 + r);
-                        cp_async<16>(dk + r * rb + o, kb0 + sl * p.k_tok + o);
-                        cp_async<16>(dv + r * rb + o, vb0 + sl * p.v_tok + o);
+                        copy_async<16>(dst + r * rb + o, src + slot(u0 + r) * tok + o);
                     }
                 }
                 if constexpr (Q4) {
                     constexpr int SC = EX ? Cfg::SROW : 4;  // bytes a copy
-                    if (u0 + lane < u1) {
-                        uint8_t* dst = dk + 2 * UNIT * Cfg::ROW + lane * sb;
-                        const int64_t src = s * p.s_seq + hk * p.s_head + slot(u0 + lane) * sb;
+                    const int u = c * UNIT + lane;
+                    if (u < total) {
+                        const uint32_t d = dst + UNIT * Cfg::ROW + lane * sb;
+                        const uint8_t* x = (const uint8_t*)(n & 1 ? a.v_scale : a.k_scale) + s0 + slot(u) * sb;
 #pragma unroll
                         for (int e = 0; e < Cfg::SROW / SC; ++e)
-                            if (SC * e < sb) {
-                                cp_async<SC>(dst + SC * e, (const uint8_t*)a.k_scale + src + SC * e);
-                                cp_async<SC>(dst + UNIT * Cfg::SROW + SC * e, (const uint8_t*)a.v_scale + src + SC * e);
-                            }
+                            if (SC * e < sb) copy_async<SC>(d + SC * e, x + SC * e);
                     }
                 }
             }
-            cp_async_commit();
+            if (Q4 || !CACHED) cp_async_commit();
+        };
+        // the slot to be read next has landed
+        auto landed = [&] {
+            if (CACHED) wait_bytes(bar + st * 8, parity, p.err);
+            if (Q4 || !CACHED) cp_async_wait<SLOTS - 1>();
+            __syncwarp();
+        };
+        auto next = [&] {
+            __syncwarp();  // every lane has read the slot
+            st = after(st, 1);
+            parity ^= st == 0;
         };
 #pragma unroll
-        for (int n = 0; n < SLOTS - 1; ++n) fetch(c0 + n, use + n);
+        for (int n = 0; n < SLOTS - 1; ++n) fetch(n, after(st, n));
 
         const RowKeys ka = row_keys<CACHED>(a, tk, r0, g, rows), kb = HALF ? ka : row_keys<CACHED>(a, tk, r0, g + 8, rows);
         // [full_lo, full_hi): every row of the tile sees these
@@ -270,7 +376,7 @@ __global__ void __launch_bounds__(StepCfg<DP, Q4>::WARPS * 32, 1) attend_step_ke
         uint32_t q[KS][4];
         auto load_q = [&](int r, int hi) {
             const bool on = r < rows;
-            const int i = on ? (r0 + r) / a.G : 0, h = hk * a.G + (on ? (r0 + r) - i * a.G : 0);
+            const int i = on ? (int)a.by_G.div(r0 + r) : 0, h = hk * a.G + (on ? (r0 + r) - i * a.G : 0);
             const T* x = (const T*)a.q + s * a.q_seq + (int64_t)i * a.q_tok + (int64_t)h * a.q_head;
 #pragma unroll
             for (int c = 0; c < KS / 2; ++c) {  // 8 channels: two contraction steps
@@ -308,16 +414,12 @@ __global__ void __launch_bounds__(StepCfg<DP, Q4>::WARPS * 32, 1) attend_step_ke
             for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
         float ma = -INFINITY, mb = -INFINITY, la = 0.f, lb = 0.f;  // rows g and g + 8: offset (log2 units), sum
 
-        for (int c = c0; c < c1; ++c, ++use) {
-            fetch(c + SLOTS - 1, use + SLOTS - 1);  // into the slot read last, while this unit is worked on
-            if (p.packed && !__all_sync(0xffffffffu, mbar_wait(&bar[use % SLOTS], use / SLOTS & 1, p.err))) return;
-            cp_async_wait<SLOTS - 1>();
-            __syncwarp();
-            const uint8_t* kp = ring + (use % SLOTS) * Cfg::SLOT;
-            const uint8_t* vp = kp + UNIT * Cfg::ROW;
-            const uint8_t* ksp = vp + UNIT * Cfg::ROW;
-            const uint8_t* vsp = ksp + UNIT * Cfg::SROW;
-            const int u0 = c * UNIT;
+        for (int n = 0; n < copies; n += 2) {
+            fetch(n + SLOTS - 1, after(st, SLOTS - 1));  // into the slot read last, while this one is worked on
+            landed();
+            const uint32_t kp = ring + st * Cfg::SLOT + g * rb + (Q4 ? DP / 8 * t : 16 * t);
+            const uint32_t ksp = ring + st * Cfg::SLOT + UNIT * Cfg::ROW + g * sb + DP / 4 * t / kGroup * 4;
+            const int u0 = (c0 + ((n >> 1) << p.inner_log2)) * UNIT;
             const bool full = u0 >= full_lo && u0 + UNIT <= full_hi;  // every row sees every key
             // ---- S = Q K^T: key tile j holds keys 8j + g ----
             float sc[JT][4];
@@ -325,20 +427,20 @@ __global__ void __launch_bounds__(StepCfg<DP, Q4>::WARPS * 32, 1) attend_step_ke
 #pragma unroll
             for (int j = 0; j < JT; ++j) {
                 sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
-                const uint8_t* row = kp + (8 * j + g) * rb;
+                const uint32_t row = kp + 8 * j * rb;
                 sm[j] = 0u;
                 if constexpr (Q4) {
 #pragma unroll
                     for (int w = 0; w < DP / 32; ++w) kx[j][w] = 0u;
                     if (EX || DP / 4 * t < D) {
-                        load_words<DP / 8>(kx[j], row + DP / 8 * t);
-                        sm[j] = *reinterpret_cast<const uint32_t*>(ksp + (8 * j + g) * sb + DP / 4 * t / kGroup * 4);
+                        load_words<DP / 8>(kx[j], row);
+                        load_words<4>(&sm[j], ksp + 8 * j * sb);
                     }
                 } else {
 #pragma unroll
                     for (int w = 0; w < KS / 2; ++w) {
                         kx[j][4 * w] = kx[j][4 * w + 1] = kx[j][4 * w + 2] = kx[j][4 * w + 3] = 0u;
-                        if (EX || 32 * w + 8 * t < D) load_words<16>(kx[j] + 4 * w, row + 64 * w + 16 * t);
+                        if (EX || 32 * w + 8 * t < D) load_words<16>(kx[j] + 4 * w, row + 64 * w);
                     }
                 }
             }
@@ -351,13 +453,15 @@ __global__ void __launch_bounds__(StepCfg<DP, Q4>::WARPS * 32, 1) attend_step_ke
                     for (int j = 0; j < JT; ++j) {
                         if constexpr (Q4) {
                             const uint32_t step = __byte_perm(sm[j], 0, 0x1010), off = __byte_perm(sm[j], 0, 0x3232);
-                            mma16816(sc[j], q[2 * w + half], widen(kx[j][w], 2 * half, step, off, (T*)nullptr),
-                                     widen(kx[j][w], 2 * half + 1, step, off, (T*)nullptr), (T*)nullptr);
+                            mma16816(sc[j], q[2 * w + half], widen(kx[j][w], 2 * half, step, off, wd),
+                                     widen(kx[j][w], 2 * half + 1, step, off, wd), (T*)nullptr);
                         } else {
                             mma16816(sc[j], q[2 * w + half], kx[j][4 * w + 2 * half], kx[j][4 * w + 2 * half + 1],
                                      (T*)nullptr);
                         }
                     }
+            next();
+            fetch(n + SLOTS, after(st, SLOTS - 1));
             if (!full) {  // unseen keys get -inf
 #pragma unroll
                 for (int j = 0; j < JT; ++j)
@@ -418,6 +522,9 @@ __global__ void __launch_bounds__(StepCfg<DP, Q4>::WARPS * 32, 1) attend_step_ke
             }
             la += ra;
             lb += rbs;
+            landed();
+            const uint32_t vp = ring + st * Cfg::SLOT + 2 * t * rb + (Q4 ? DP / 16 : DP / 4) * g;
+            const uint32_t vsp = ring + st * Cfg::SLOT + UNIT * Cfg::ROW + 2 * t * sb + DP / 8 * g / kGroup * 4;
             // ---- O += P V, 16 keys at a time: values 2t, 2t + 1, 8 + 2t, 9 + 2t ----
 #pragma unroll
             for (int h = 0; h < UNIT / 16; ++h) {
@@ -426,23 +533,36 @@ __global__ void __launch_bounds__(StepCfg<DP, Q4>::WARPS * 32, 1) attend_step_ke
                 uint32_t v[4][W], vs[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int kr = 16 * h + 2 * t + 8 * (j >> 1) + (j & 1);
-                    const uint8_t* row = vp + kr * rb;
-                    const bool on = full || u0 + kr < total;  // rows past the last key hold anything
+                    const int kr = 16 * h + 8 * (j >> 1) + (j & 1);
+                    const uint32_t row = vp + kr * rb;
+                    if constexpr (!EX) {
 #pragma unroll
-                    for (int w = 0; w < W; ++w) v[j][w] = 0u;
-                    vs[j] = 0u;
+                        for (int w = 0; w < W; ++w) v[j][w] = 0u;
+                        vs[j] = 0u;
+                    }
                     if constexpr (Q4) {
-                        if (on && (EX || DP / 8 * g < D)) {
-                            load_words<DP / 16>(v[j], row + DP / 16 * g);
-                            vs[j] = *reinterpret_cast<const uint32_t*>(vsp + kr * sb + DP / 8 * g / kGroup * 4);
+                        if (EX || DP / 8 * g < D) {
+                            load_words<DP / 16>(v[j], row);
+                            load_words<4>(&vs[j], vsp + kr * sb);
                         }
                     } else if constexpr (DP == 32) {
-                        if (on && (EX || 4 * g < D)) load_words<8>(v[j], row + 8 * g);
+                        if (EX || 4 * g < D) load_words<8>(v[j], row);
                     } else {
 #pragma unroll
                         for (int w = 0; w < DP / 64; ++w)
-                            if (on && (EX || DP / 8 * g + 8 * w < D)) load_words<16>(v[j] + 4 * w, row + DP / 4 * g + 16 * w);
+                            if (EX || DP / 8 * g + 8 * w < D) load_words<16>(v[j] + 4 * w, row + 16 * w);
+                    }
+                }
+                if (!full) {  // rows past the last key hold anything: zeros instead (4 bits: by step and offset)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const bool on = u0 + 16 * h + 2 * t + 8 * (j >> 1) + (j & 1) < total;
+                        if constexpr (Q4) {
+                            vs[j] = on ? vs[j] : 0u;
+                        } else {
+#pragma unroll
+                            for (int w = 0; w < W; ++w) v[j][w] = on ? v[j][w] : 0u;
+                        }
                     }
                 }
                 if constexpr (Q4) {
@@ -459,8 +579,8 @@ __global__ void __launch_bounds__(StepCfg<DP, Q4>::WARPS * 32, 1) attend_step_ke
                         const uint32_t hi = __byte_perm(v[2][w >> 1], v[3][w >> 1], sel);
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            mma16816(o[4 * w + i], pa, widen(lo, i, step[0], off[0], (T*)nullptr),
-                                     widen(hi, i, step[1], off[1], (T*)nullptr), (T*)nullptr);
+                            mma16816(o[4 * w + i], pa, widen(lo, i, step[0], off[0], wd),
+                                     widen(hi, i, step[1], off[1], wd), (T*)nullptr);
                     }
                 } else {
 #pragma unroll
@@ -472,7 +592,7 @@ __global__ void __launch_bounds__(StepCfg<DP, Q4>::WARPS * 32, 1) attend_step_ke
                     }
                 }
             }
-            __syncwarp();  // the slot is read
+            next();
         }
 
         // ---- this part's result; accumulator column 2t, 2t + 1 of tile i is channel NT * 2t + i, NT * (2t + 1) + i ----
@@ -480,95 +600,87 @@ __global__ void __launch_bounds__(StepCfg<DP, Q4>::WARPS * 32, 1) attend_step_ke
         la += __shfl_xor_sync(0xffffffffu, la, 2);
         lb += __shfl_xor_sync(0xffffffffu, lb, 1);
         lb += __shfl_xor_sync(0xffffffffu, lb, 2);
+        // The group's results are joined through its warps' rings, whose copies have all landed and are read.
+        constexpr int LD = DP + 2;  // a row's sums, its offset and sum
         auto put = [&](int r, int e, float m, float l) {
-            if (r >= rows) return;
-            const int64_t row = seg * p.rows + r;
-            if (t == 0) p.part_ml[row] = make_float2(m, l);
-            float4* dst = reinterpret_cast<float4*>(p.part_o + row * DP + 2 * NT * t);
+            float* dst = reinterpret_cast<float*>(smem + warp * Cfg::RING) + r * LD;
 #pragma unroll
-            for (int i = 0; i < NT / 4; ++i) {
-                dst[i] = make_float4(o[4 * i][e], o[4 * i + 1][e], o[4 * i + 2][e], o[4 * i + 3][e]);
-                dst[NT / 4 + i] =
-                    make_float4(o[4 * i][e + 1], o[4 * i + 1][e + 1], o[4 * i + 2][e + 1], o[4 * i + 3][e + 1]);
+            for (int i = 0; i < NT; ++i) {
+                dst[2 * NT * t + i] = o[i][e];
+                dst[2 * NT * t + NT + i] = o[i][e + 1];
             }
+            if (t == 0) dst[DP] = m, dst[DP + 1] = l;
         };
-        put(g, 0, ma, la);
-        if constexpr (!HALF) put(g + 8, 2, mb, lb);
+        if (g < rows) put(g, 0, ma, la);
+        if constexpr (!HALF) {
+            if (g + 8 < rows) put(g + 8, 2, mb, lb);
+        }
+        auto group_sync = [&] {
+            if (inner > 1) asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(inner * 32) : "memory");
+            else __syncwarp();
+        };
+        group_sync();
+        const float* first = reinterpret_cast<const float*>(smem + (warp - part) * Cfg::RING);
+        for (int r = part; r < rows; r += inner) {
+            float top = -INFINITY, l = 0.f, v[DP / 32];
+            for (int b = 0; b < inner; ++b) top = fmaxf(top, first[b * (Cfg::RING / 4) + r * LD + DP]);
+#pragma unroll
+            for (int e = 0; e < DP / 32; ++e) v[e] = 0.f;
+            for (int b = 0; b < inner; ++b) {
+                const float* x = first + b * (Cfg::RING / 4) + r * LD;
+                const float f = to_offset(x[DP], top);
+                l += f * x[DP + 1];
+#pragma unroll
+                for (int e = 0; e < DP / 32; ++e) v[e] += f * x[lane + 32 * e];
+            }
+            if (p.outer == 1) {
+                finish_row<T, DP, Q4, CACHED>(a, tk, row_keys<CACHED>(a, tk, r0, r, rows), s, hk, r0 + r, v, l);
+            } else {
+                const int64_t row = (int64_t)seg * p.rows + r;
+#pragma unroll
+                for (int e = 0; e < DP / 32; ++e) p.part_o[row * DP + lane + 32 * e] = v[e];
+                if (lane == 0) p.part_ml[row] = make_float2(top, l);
+            }
+        }
+        fence_async_smem();  // before the next item's copies overwrite what was written and read here
+        group_sync();
     }
 }
 
-// Joins the parts of each row: wpr warps a row (1, 2, 4 or 8), 8 / wpr rows a CTA.
+// Joins the shares of each row, one warp a row.
 template <typename T, int DP, bool Q4, bool CACHED>
-__global__ void __launch_bounds__(256) join_step_kernel(const StepArgs p, int wpr, int tile_rows) {
-    __shared__ float s_o[8][DP];
-    __shared__ float s_l[8];
+__global__ void __launch_bounds__(128) join_step_kernel(const StepArgs p, int tile_rows) {
     const AttnArgs& a = p.a;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp % wpr;
-    const int64_t n = p.items * p.rows, at = (int64_t)blockIdx.x * (8 / wpr) + warp / wpr;
-    const int64_t item = at / p.rows;
+    const int lane = threadIdx.x & 31;
+    const unsigned at = blockIdx.x * 4 + (threadIdx.x >> 5), item = at / (unsigned)p.rows;
     const int r = (int)(at - item * p.rows);
-    const int64_t hs = item / p.tiles;
-    const int r0 = (int)(item - hs * p.tiles) * tile_rows;
-    const int64_t s = hs / a.Hkv;
-    const int hk = (int)(hs - s * a.Hkv), rows = min(tile_rows, a.Nq * a.G - r0);
-    const bool on = at < n && r < rows;
-    const int i = on ? (r0 + r) / a.G : 0, h = hk * a.G + (on ? (r0 + r) - i * a.G : 0);
+    const unsigned hs = p.by_tiles.div(item), sq = a.by_Hkv.div(hs);
+    const int r0 = (int)(item - hs * p.tiles) * tile_rows, rows = min(tile_rows, a.Nq * a.G - r0);
+    const bool on = item < p.items && r < rows;
     TileKeys tk{};
     RowKeys k{0, 0, 0};
-    float gate = 1.f;
     if (on) {
-        tk = tile_keys<CACHED>(a, s, r0, rows);
+        tk = tile_keys<CACHED>(a, sq, r0, rows);
         k = row_keys<CACHED>(a, tk, r0, r, rows);
-        if (a.gates) gate = __ldg(a.gates + (s * a.Nq + i) * a.Hq + h);
     }
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // the parts are written
-    float l = 0.f, v[DP / 32];
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the shares are written
+    if (!on) return;
+    const int64_t row0 = (int64_t)item * p.outer * p.rows + r;
+    float top = -INFINITY, l = 0.f, v[DP / 32];
 #pragma unroll
     for (int e = 0; e < DP / 32; ++e) v[e] = 0.f;
-    if (on) {
-        const int64_t row0 = item * p.parts * p.rows + r;
-        float top = -INFINITY;
-        for (int b = lane; b < p.parts; b += 32) top = fmaxf(top, p.part_ml[row0 + (int64_t)b * p.rows].x);
-        top = warp_max(top);
-#pragma unroll 4
-        for (int b = sub; b < p.parts; b += wpr) {
-            const int64_t row = row0 + (int64_t)b * p.rows;
-            const float2 ml = p.part_ml[row];
-            const float f = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - top);
-            l += f * ml.y;
+    for (int b = lane; b < p.outer; b += 32) top = fmaxf(top, p.part_ml[row0 + (int64_t)b * p.rows].x);
+    top = warp_max(top);
+#pragma unroll 8
+    for (int b = 0; b < p.outer; ++b) {
+        const int64_t row = row0 + (int64_t)b * p.rows;
+        const float2 ml = p.part_ml[row];
+        const float f = to_offset(ml.x, top);
+        l += f * ml.y;
 #pragma unroll
-            for (int e = 0; e < DP / 32; ++e) v[e] += f * p.part_o[row * DP + lane + 32 * e];
-        }
+        for (int e = 0; e < DP / 32; ++e) v[e] += f * p.part_o[row * DP + lane + 32 * e];
     }
-    if (wpr > 1) {
-#pragma unroll
-        for (int e = 0; e < DP / 32; ++e) s_o[warp][lane + 32 * e] = v[e];
-        if (lane == 0) s_l[warp] = l;
-        __syncthreads();
-        if (sub == 0)
-            for (int w = 1; w < wpr; ++w) {
-                l += s_l[warp + w];
-#pragma unroll
-                for (int e = 0; e < DP / 32; ++e) v[e] += s_o[warp + w][lane + 32 * e];
-            }
-    }
-    if (!on || sub != 0) return;
-    const bool sees = k.f > 0 || k.b > k.a;
-    const float inv = sees ? gate / l : 0.f;
-    bool bad = false;
-#pragma unroll
-    for (int e = 0; e < DP / 32; ++e) {
-        v[e] = sees ? v[e] * inv : 0.f;
-        bad |= lane + 32 * e < a.D && !isfinite(v[e]);
-    }
-    if (__any_sync(0xffffffffu, bad)) {
-        attend_row<T, CACHED, Q4>(a, s, i, h, tk.n, tk.m);
-    } else {
-        T* out = (T*)a.out + s * a.o_seq + (int64_t)i * a.o_tok + (int64_t)h * a.o_head;
-#pragma unroll
-        for (int e = 0; e < DP / 32; ++e)
-            if (lane + 32 * e < a.D) out[lane + 32 * e] = from_f32<T>(v[e]);
-    }
+    finish_row<T, DP, Q4, CACHED>(a, tk, k, sq, (int)(hs - sq * a.Hkv), r0 + r, v, l);
 }
 
 int sm_count() {
@@ -588,21 +700,20 @@ void launch(const StepArgs& p, cudaStream_t st) {
         MBR_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::TOTAL));
         attr[dev] = true;
     }
-    const int64_t segs = p.items * p.parts;
-    const unsigned grid = (unsigned)std::min<int64_t>(segs, sm_count());
+    const unsigned grid = (unsigned)std::min<int64_t>((int64_t)p.items * p.outer, sm_count());
     kern<<<grid, Cfg::WARPS * 32, Cfg::TOTAL, st>>>(p);
     MBR_CUDA(cudaGetLastError());
-    const int wpr = p.parts <= 8 ? 1 : p.parts <= 16 ? 2 : p.parts <= 32 ? 4 : 8;  // at most about eight parts a warp
+    if (p.outer == 1) return;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)ceil_div(p.items * p.rows, 8 / wpr));
-    cfg.blockDim = dim3(256);
+    cfg.gridDim = dim3((unsigned)ceil_div((int64_t)p.items * p.rows, 4));
+    cfg.blockDim = dim3(128);
     cfg.stream = st;
     cudaLaunchAttribute at;
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    MBR_CUDA(cudaLaunchKernelEx(&cfg, join_step_kernel<T, DP, Q4, CACHED>, p, wpr, HALF ? 8 : 16));
+    MBR_CUDA(cudaLaunchKernelEx(&cfg, join_step_kernel<T, DP, Q4, CACHED>, p, HALF ? 8 : 16));
 }
 
 template <typename T, bool Q4, bool CACHED, bool HALF>
@@ -634,31 +745,37 @@ StepPlan step_plan(int64_t seqs, int64_t tokens, int Hq, int Hkv, int D, int64_t
     pl.rows = (int)std::min<int64_t>(rows, 16);
     pl.tiles = ceil_div(rows, 16);
     pl.items = seqs * Hkv * pl.tiles;
-    const int dp = D == 32 ? 32 : D == 64 ? 64 : 128;
-    const int64_t warps = 148 * (dp == 128 ? 8 : 16);
-    // Parts: the time of a warp is rounds x (its part's keys + a start worth about
-    // 64 keys); the join reads every part, so it has a price too.
-    double best = 0.;
-    pl.parts = 1;
-    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(512, keys / 32));
-    for (int64_t n = 1; n <= most && pl.items * n <= (1 << 24); ++n) {
-        const double cost = (double)ceil_div(pl.items * n, warps) * ((double)keys / n + 64.) + 0.5 * n;
-        if (n == 1 || cost < best) best = cost, pl.parts = (int)n;
-    }
-    pl.bytes = pl.items * pl.parts * pl.rows * (int64_t)(dp + 2) * 4;
+    const int dp = D == 32 ? 32 : D == 64 ? 64 : 128, warps = step_warps(dp);
+    // A warp's time is its rounds x (its keys + a start and a join worth some 100
+    // keys).  One CTA an item joins inside; more CTAs cost a second kernel (some
+    // 500 keys) and the reading of each share.
+    double best = 1e300;
+    auto consider = [&](int inner, int outer) {
+        const double rounds = (double)ceil_div(pl.items * outer, (int64_t)148 * (warps / inner));
+        const double cost = rounds * ((double)keys / inner / outer + 100.) + (outer > 1 ? 500. + 10. * outer : 0.);
+        if (cost < best) best = cost, pl.inner = inner, pl.outer = outer;
+    };
+    for (int n = 1; n <= warps; n *= 2) consider(n, 1);
+    for (int n = 2; n <= std::min<int64_t>(148, keys / UNIT / warps); ++n)
+        if (pl.items * n <= 148 * 4) consider(warps, n);
+    pl.bytes = pl.outer == 1 ? 0 : pl.items * pl.outer * pl.rows * (int64_t)(dp + 2) * 4;
     return pl;
 }
 
 void attend_step(const AttnArgs& a, int dtype, bool cached, bool q4, const StepPlan& pl, void* workspace,
                  cudaStream_t st) {
     MBR_CHECK(((uintptr_t)workspace & 15) == 0, "attention: workspace must be 16-byte aligned");
+    MBR_CHECK(pl.items < (1ll << 27), "attention: too many row tiles");
     StepArgs p{};
     p.a = a;
     p.scale_log2 = a.scale * 1.4426950408889634f;
-    p.items = pl.items, p.tiles = pl.tiles, p.parts = pl.parts, p.rows = pl.rows, p.half = pl.half;
+    p.items = (unsigned)pl.items, p.tiles = (int)pl.tiles, p.rows = pl.rows, p.half = pl.half;
+    p.outer = pl.outer;
+    while ((1 << p.inner_log2) < pl.inner) ++p.inner_log2;
+    p.by_tiles = FastDiv((unsigned)pl.tiles), p.by_outer = FastDiv((unsigned)pl.outer);
     const int dp = a.D == 32 ? 32 : a.D == 64 ? 64 : 128;
     p.part_o = (float*)workspace;
-    p.part_ml = (float2*)(p.part_o + pl.items * pl.parts * pl.rows * dp);
+    p.part_ml = (float2*)(p.part_o + pl.items * pl.outer * pl.rows * dp);
     p.q_vec = (((uintptr_t)a.q & 15) == 0 && (a.q_seq | a.q_tok | a.q_head) % 8 == 0) ? 1 : 0;
     const int64_t es = 2;
     if (cached) {
@@ -671,7 +788,6 @@ void attend_step(const AttnArgs& a, int dtype, bool cached, bool q4, const StepP
         p.k_tok = a.k_tok * es, p.k_head = a.k_head * es, p.k_seq = a.k_seq * es;
         p.v_tok = a.v_tok * es, p.v_head = a.v_head * es, p.v_seq = a.v_seq * es;
     }
-    p.packed = p.k_tok == (q4 ? a.D / 2 : a.D * es) && p.v_tok == p.k_tok;
     p.err = stream_error_word();
     if (dtype == DT_BF16) {
         if (!cached) dispatch<__nv_bfloat16, false, false>(p, st);

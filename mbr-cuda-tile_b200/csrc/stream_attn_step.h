@@ -6,28 +6,31 @@
 namespace mbr {
 namespace streamops {
 
-// How a call is divided: items are (sequence, key head, row tile), each walked
-// in `parts` parts whose results lie in the workspace.
+// How a call is divided.  Items are (sequence, key head, row tile); `outer` CTAs
+// share an item's keys, and in each of them a group of `inner` warps (a power of
+// two).
 struct StepPlan {
     int64_t items, tiles;
-    int parts, rows;  // rows: of a tile
-    bool half;        // at most 8 rows
-    int64_t bytes;    // workspace
+    int inner, outer, rows;  // rows: of a tile
+    bool half;               // at most 8 rows
+    int64_t bytes;           // workspace: the results of `outer` CTAs, which a second kernel joins (0: none)
 };
 // keys: the most keys any tile can see.
 StepPlan step_plan(int64_t seqs, int64_t tokens, int Hq, int Hkv, int D, int64_t keys);
+// Warps of a CTA (one CTA an SM) for a head size of up to dp.
+constexpr int step_warps(int dp) { return dp == 128 ? 8 : 16; }
 
 struct StepArgs {
     AttnArgs a;
     // byte strides of key, value and (4 bits) step/offset rows
     int64_t k_seq, k_head, k_tok, v_seq, v_head, v_tok, s_seq, s_head;
     float scale_log2;  // scale * log2(e)
-    int64_t items, tiles;
-    int parts, rows, half;
+    unsigned items;
+    int tiles, inner_log2, outer, rows, half;
+    FastDiv by_tiles, by_outer;
     int q_vec;        // query rows are 16-byte aligned
-    int packed;       // a token's row follows the one before it
-    float* part_o;    // [items * parts][rows][DP]
-    float2* part_ml;  // [items * parts][rows] (offset, sum)
+    float* part_o;    // [items * outer][rows][DP]
+    float2* part_ml;  // [items * outer][rows] (offset, sum)
     int* err;         // error word of bounded waits
 };
 
