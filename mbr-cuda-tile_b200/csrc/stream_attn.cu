@@ -5,6 +5,7 @@
 
 #include "stream_attn.cuh"
 #include "stream_attn_step.h"
+#include "stream_attn_tc.h"
 
 namespace mbr {
 namespace streamops {
@@ -139,6 +140,10 @@ void window_attention(const mbr_view& q, const mbr_view& k, const mbr_view& v, c
         const StepPlan pl = plan_of(a, Nk);
         MBR_CHECK(pl.bytes == 0 || (workspace && workspace_bytes >= pl.bytes), "window_attention: workspace too small");
         attend_step(a, dtype, false, false, pl, workspace, st);
+        return;
+    }
+    if (tile_supported(a, dtype)) {
+        attend_tiles(a, dtype, st);
         return;
     }
     launch_rows<false>(a, dtype, false, st);
