@@ -43,15 +43,16 @@ using namespace sm100;
 constexpr int QROWS = 128, KB = 64;
 constexpr float kRescaleSum = 16384.0f;
 
-// Shared memory of a CTA: Q, two stages of K and of V (64-channel halves of 128-byte rows, 128-byte swizzle), barriers.
+// Shared memory of a CTA: Q, NS stages of K and of V (64-channel halves of 128-byte rows, 128-byte swizzle), barriers.
 template <int DH>
 struct TileCfg {
+    static constexpr int NS = DH == 1 ? 3 : 2;
     static constexpr int Q = 0;
     static constexpr int K = DH * 16384;
-    static constexpr int V = K + 2 * DH * 8192;
-    static constexpr int BAR = V + 2 * DH * 8192;
+    static constexpr int V = K + NS * DH * 8192;
+    static constexpr int BAR = V + NS * DH * 8192;
     static constexpr int TOTAL = BAR + 128;
-    static constexpr int CTAS = DH == 1 ? 4 : 2;  // an SM
+    static constexpr int CTAS = DH == 1 ? 3 : 2;  // an SM
     static constexpr uint32_t TMEM = DH == 1 ? 128 : 256;
     static constexpr uint32_t O = 64;  // S at column 0, O behind it
     static_assert(CTAS * (TOTAL + 1024) <= 233472, "CTAs an SM");
@@ -135,17 +136,18 @@ __global__ void __launch_bounds__(160, TileCfg<DH>::CTAS)
     extern __shared__ __align__(1024) uint8_t sm[];
     if (!smem_aligned_or_flag(sm, p.err)) return;  // uniform over the CTA
     uint64_t* bar = (uint64_t*)(sm + Cfg::BAR);
-    uint64_t* bar_q = bar;      // Q landed
-    uint64_t* bar_k = bar + 1;  // [2] K stage landed
-    uint64_t* bar_v = bar + 3;  // [2] V stage landed
-    uint64_t* bar_s = bar + 5;  // S of the next block computed (and every product issued before it)
-    uint64_t* bar_p = bar + 6;  // P written, S read (4 warps)
-    uint64_t* bar_o = bar + 7;  // a tile's last product done
-    uint32_t* tmem_slot = (uint32_t*)(bar + 8);
+    constexpr int NS = Cfg::NS;
+    uint64_t* bar_q = bar;           // Q landed
+    uint64_t* bar_s = bar + 1;       // S of the next block computed (and every product issued before it)
+    uint64_t* bar_o = bar + 2;       // a tile's last product done
+    uint64_t* bar_p = bar + 3;       // P written, S read (4 warps)
+    uint64_t* bar_k = bar + 4;       // [NS] K stage landed
+    uint64_t* bar_v = bar_k + NS;    // [NS] V stage landed
+    uint32_t* tmem_slot = (uint32_t*)(bar_v + NS);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 8; ++i) mbar_init(&bar[i], i == 6 ? 4 : 1);
+        for (int i = 0; i < 4 + 2 * NS; ++i) mbar_init(&bar[i], i == 3 ? 4 : 1);
         fence_barrier_init();
     }
     if (warp == 4) {
@@ -159,7 +161,7 @@ __global__ void __launch_bounds__(160, TileCfg<DH>::CTAS)
 
     if (warp == 4) {
         // ---- loads and products; one lane issues, all wait ----
-        // The blocks of all of this CTA's tiles form one stream g; K(g) and V(g) go through stage g % 2.
+        // The blocks of all of this CTA's tiles form one stream g; K(g) and V(g) go through stage g % NS.
         struct Block {
             int key, hk, s;  // coordinates
             int left;        // keys of the sequence from here on
@@ -192,19 +194,17 @@ __global__ void __launch_bounds__(160, TileCfg<DH>::CTAS)
 #pragma unroll
             for (int h = 0; h < DH; ++h) tma_load_4d(sm + Cfg::Q + h * 16384, &tmQ, 64 * h, b.h0, b.tok0, b.s, bar_q);
         };
-        auto load_k = [&](const Block& b, int g) {
-            uint64_t* br = &bar_k[g & 1];
-            mbar_arrive_expect_tx(br, DH * 8192);
+        auto load_k = [&](const Block& b, int st) {
+            mbar_arrive_expect_tx(&bar_k[st], DH * 8192);
 #pragma unroll
             for (int h = 0; h < DH; ++h)
-                tma_load_4d(sm + Cfg::K + ((g & 1) * DH + h) * 8192, &tmK, 64 * h, b.hk, b.key, b.s, br);
+                tma_load_4d(sm + Cfg::K + (st * DH + h) * 8192, &tmK, 64 * h, b.hk, b.key, b.s, &bar_k[st]);
         };
-        auto load_v = [&](const Block& b, int g) {
-            uint64_t* br = &bar_v[g & 1];
-            mbar_arrive_expect_tx(br, DH * 8192);
+        auto load_v = [&](const Block& b, int st) {
+            mbar_arrive_expect_tx(&bar_v[st], DH * 8192);
 #pragma unroll
             for (int h = 0; h < DH; ++h)
-                tma_load_4d(sm + Cfg::V + ((g & 1) * DH + h) * 8192, &tmV, 64 * h, b.hk, b.key, b.s, br);
+                tma_load_4d(sm + Cfg::V + (st * DH + h) * 8192, &tmV, 64 * h, b.hk, b.key, b.s, &bar_v[st]);
         };
         auto wait_all = [&](uint64_t* b, uint32_t parity) {
             return __all_sync(0xffffffffu, mbar_wait(b, parity, p.err));
@@ -215,13 +215,20 @@ __global__ void __launch_bounds__(160, TileCfg<DH>::CTAS)
         const uint64_t dK = sdesc_sw128(smem_u32(sm + Cfg::K));
         const uint64_t dV = sdesc_sw128_mn(smem_u32(sm + Cfg::V));
         const int ksteps = (p.a.D + 15) / 16;  // channels past the head size are zeros: no product for whole steps of them
-        auto issue_s = [&](int g) {
-            const uint64_t k0 = dK + (uint64_t)(512 * DH * (g & 1));
-            for (int k = 0; k < ksteps; ++k)  // 32 bytes a step, 16 KB (Q) or 8 KB (K) a half
-                mma_f16(tmem, dQ + 1024 * (k >> 2) + 2 * (k & 3), k0 + 512 * (k >> 2) + 2 * (k & 3), idS, k > 0);
+        auto issue_s = [&](int st) {  // 32 bytes a step, 16 KB (Q) or 8 KB (K) a half
+            const uint64_t k0 = dK + (uint64_t)(512 * DH * st);
+            if (ksteps == 4 * DH) {
+#pragma unroll
+                for (int k = 0; k < 4 * DH; ++k)
+                    mma_f16(tmem, dQ + 1024 * (k >> 2) + 2 * (k & 3), k0 + 512 * (k >> 2) + 2 * (k & 3), idS, k > 0);
+            } else {
+                for (int k = 0; k < ksteps; ++k)
+                    mma_f16(tmem, dQ + 1024 * (k >> 2) + 2 * (k & 3), k0 + 512 * (k >> 2) + 2 * (k & 3), idS, k > 0);
+            }
+            mma_commit(bar_s);
         };
-        auto issue_pv = [&](int g, bool first) {
-            const uint64_t v0 = dV + (uint64_t)(512 * DH * (g & 1));
+        auto issue_pv = [&](int st, bool first) {
+            const uint64_t v0 = dV + (uint64_t)(512 * DH * st);
 #pragma unroll
             for (int h = 0; h < DH; ++h)
 #pragma unroll
@@ -229,66 +236,83 @@ __global__ void __launch_bounds__(160, TileCfg<DH>::CTAS)
                     mma_f16_ts(tmem + Cfg::O + 64 * h, tmem + 8 * k, v0 + 512 * h + 128 * k, idO, !first || k > 0);
         };
 
-        Block b0 = next_block(), b1 = next_block();
+        Block b[NS];  // blocks g .. g + NS - 1
+#pragma unroll
+        for (int i = 0; i < NS; ++i) b[i] = next_block();
         if (lane == 0) {
             prefetch_tensormap(&tmQ);
             prefetch_tensormap(&tmK);
             prefetch_tensormap(&tmV);
-            if (b0.any) load_q(b0), load_k(b0, 0), load_v(b0, 0);
-            if (b1.any) load_k(b1, 1), load_v(b1, 1);
+            if (b[0].any) load_q(b[0]);
+#pragma unroll
+            for (int i = 0; i < NS; ++i)
+                if (b[i].any) load_k(b[i], i), load_v(b[i], i);
         }
         __syncwarp();
-        uint32_t qphase = 0;
         bool ok = true;
-        if (b0.any) {
+        uint32_t qphase = 1;  // of the next tile's Q
+        bool behind = false;  // there is a block g - 1
+        if (b[0].any) {
             ok = wait_all(bar_q, 0) && wait_all(&bar_k[0], 0);
-            qphase = 1;
             if (ok) {
                 tc_fence_after();
-                if (lane == 0) issue_s(0), mma_commit(bar_s);
+                if (lane == 0) issue_s(0);
                 __syncwarp();
             }
         }
-        for (int g = 0; b0.any && ok; ++g) {
-            const Block b2 = next_block();  // of the stage that S(g) frees
-            ok = wait_all(&bar_v[g & 1], (g >> 1) & 1);
+        // stage and parity of block g and of block g + 1
+        int st = 0, st1 = 1 % NS;
+        uint32_t par = 0, par1 = NS == 1 ? 1 : 0;
+        for (uint32_t gp = 0; b[0].any && ok; gp ^= 1) {  // gp: parity of g
+            const bool more = b[1].any, fresh = b[1].first;  // a next block; it starts another tile
+            ok = wait_all(&bar_v[st], par) && (!more || wait_all(&bar_k[st1], par1));
             if (!ok) break;
-            if (b0.left < KB) {  // rows past the sequence's length hold anything: zeros
-                const int r0 = max(b0.left, 0);
+            if (b[0].left < KB) {  // rows past the sequence's length hold anything: zeros
+                const int r0 = max(b[0].left, 0);
                 for (int i = lane; i < (KB - r0) * 8 * DH; i += 32) {
                     const int row = i >> 3, h = row / (KB - r0), r = r0 + row - h * (KB - r0);
-                    *reinterpret_cast<uint4*>(sm + Cfg::V + ((g & 1) * DH + h) * 8192 + r * 128 + (i & 7) * 16) =
+                    *reinterpret_cast<uint4*>(sm + Cfg::V + (st * DH + h) * 8192 + r * 128 + (i & 7) * 16) =
                         make_uint4(0u, 0u, 0u, 0u);
                 }
                 fence_async_smem();
                 __syncwarp();
             }
-            ok = wait_all(bar_p, g & 1);
+            ok = wait_all(bar_p, gp);
             if (!ok) break;
             tc_fence_after();
             if (lane == 0) {
-                issue_pv(g, b0.first);
-                // the next block starts another tile: this one's output is ready with this product
-                if (!b1.any || b1.first) mma_commit(bar_o);
+                issue_pv(st, b[0].first);
+                if (more && !fresh) {
+                    issue_s(st1);
+                } else {  // the tile's output is ready with this product; S(g) is done: a next tile's Q may take its place
+                    mma_commit(bar_o);
+                    if (more) load_q(b[1]);
+                }
             }
             __syncwarp();
-            // S(g) is done: a new tile's Q may take this one's place
-            if (b1.any && b1.first && lane == 0) load_q(b1);
-            if (b1.any) {
-                ok = (!b1.first || wait_all(bar_q, qphase & 1)) && wait_all(&bar_k[(g + 1) & 1], ((g + 1) >> 1) & 1);
-                if (!ok) break;
-                if (b1.first) ++qphase;
-                tc_fence_after();
-                if (lane == 0) issue_s(g + 1), mma_commit(bar_s);
-            }
+            const Block fresh_block = next_block();  // block g + NS
             if (lane == 0) {
-                // S(g) done: K(g)'s stage is free.  P.V(g - 1) was issued before S(g): V(g - 1)'s stage is free.
-                if (b2.any) load_k(b2, g + 2);
-                if (g >= 1 && b1.any) load_v(b1, g + 1);
+                // S(g) done: K(g)'s stage is free.  P.V(g - 1) was issued before S(g): V(g - 1)'s stage is free, for
+                // block g - 1 + NS.
+                if (fresh_block.any) load_k(fresh_block, st);
+                if (behind && b[NS - 1].any) load_v(b[NS - 1], st == 0 ? NS - 1 : st - 1);
             }
+            behind = true;
             __syncwarp();
-            b0 = b1;
-            b1 = b2;
+            if (more && fresh) {
+                ok = wait_all(bar_q, qphase & 1);
+                if (!ok) break;
+                ++qphase;
+                tc_fence_after();
+                if (lane == 0) issue_s(st1);
+                __syncwarp();
+            }
+#pragma unroll
+            for (int i = 0; i + 1 < NS; ++i) b[i] = b[i + 1];
+            b[NS - 1] = fresh_block;
+            st = st1, par = par1;
+            st1 = st1 + 1 == NS ? 0 : st1 + 1;
+            if (st1 == 0) par1 ^= 1;
         }
     } else {
         // ---- softmax: thread r owns row r of the tile (tensor-memory lane r) ----
@@ -297,18 +321,20 @@ __global__ void __launch_bounds__(160, TileCfg<DH>::CTAS)
         const uint32_t lanes = (uint32_t)(warp * 32) << 16;
         const uint32_t tS = tmem + lanes, tO = tmem + lanes + Cfg::O;
         const int rt = (int)p.by_pack.div(r), rh = r - rt * p.pack;  // token and head within the tile
-        const float c = fabsf(p.scale_log2);
-        const uint32_t flip = p.scale_log2 < 0.f ? 0x80000000u : 0u;  // a negative scale turns the scores' signs
+        const float c = p.scale_log2;
         int g = 0;           // blocks so far
         uint32_t tiles = 0;  // tiles with blocks so far
         bool ok = true;      // warp-uniform: tensor-memory loads and stores are warp-collective
+        Tile next = tile_at(p, blockIdx.x);
         for (unsigned t = blockIdx.x; t < p.ntiles && ok; t += gridDim.x) {
-            const Tile x = tile_at(p, t);
+            const Tile x = next;
             const int token = x.tok0 + rt;
             const bool valid = rt < p.tokens && token < a.Nq;
             Window w{0, 0, 0};
             if (valid && token < x.n) w = row_window<false>(a, token, x.n, x.m);
             const bool sees = w.hi > w.lo || w.first > 0;
+            const int h = x.h0 + rh;
+            const float gate = valid && a.gates ? __ldg(a.gates + ((int64_t)x.s * a.Nq + token) * a.Hq + h) : 1.f;
             float m = -INFINITY, l = 0.f;
             for (int j = 0; j < x.nkv; ++j, ++g) {
                 const int key = block_key(x, j);
@@ -321,37 +347,41 @@ __global__ void __launch_bounds__(160, TileCfg<DH>::CTAS)
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
                     if (__any_sync(0xffffffffu, half[q] != 0u)) need |= 1u << q;
-                    if (__all_sync(0xffffffffu, half[q] == 0xffffffffu || !sees)) whole |= 1u << q;
+                    if ((need >> q & 1) && __all_sync(0xffffffffu, half[q] == 0xffffffffu || !sees)) whole |= 1u << q;
                 }
                 ok = __all_sync(0xffffffffu, mbar_wait(bar_s, g & 1, p.err));
                 if (!ok) break;
                 tc_fence_after();
                 uint32_t pk[32];
-                // weights with offset mo as 16-bit pairs; returns this row's sum
+                // weights with offset mo as 16-bit pairs; returns this row's sum.  A chunk's scores are loaded
+                // when it comes to them: two at once would not leave registers for three CTAs.
                 auto weights = [&](float mo) {
                     float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        if (!(need >> q & 1)) {
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) pk[16 * q + i] = 0u;
-                            continue;
-                        }
-                        uint32_t sv[32];
-                        tmem_ld32(tS + 32 * q, sv);
-                        tmem_ld_wait(sv);
-                        const bool all = whole >> q & 1;
+                    uint32_t sv[32];
+                    auto chunk = [&](int q, auto all) {
 #pragma unroll
                         for (int i = 0; i < 32; i += 2) {
-                            float e0 = ex2_approx(fmaf(__uint_as_float(sv[i] ^ flip), c, -mo));
-                            float e1 = ex2_approx(fmaf(__uint_as_float(sv[i + 1] ^ flip), c, -mo));
-                            if (!all) {
+                            float e0 = ex2_approx(fmaf(__uint_as_float(sv[i]), c, -mo));
+                            float e1 = ex2_approx(fmaf(__uint_as_float(sv[i + 1]), c, -mo));
+                            if constexpr (!decltype(all)::value) {
                                 e0 = half[q] >> i & 1 ? e0 : 0.f;
                                 e1 = half[q] >> (i + 1) & 1 ? e1 : 0.f;
                             }
                             sum[i & 2] += e0;
                             sum[(i & 2) + 1] += e1;
                             pk[16 * q + i / 2] = pack2(e0, e1, (T*)nullptr);
+                        }
+                    };
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        if (need >> q & 1) {
+                            tmem_ld32(tS + 32 * q, sv);
+                            tmem_ld_wait(sv);
+                            if (whole >> q & 1) chunk(q, std::true_type{});
+                            else chunk(q, std::false_type{});
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) pk[16 * q + i] = 0u;
                         }
                     }
                     return (sum[0] + sum[1]) + (sum[2] + sum[3]);
@@ -372,7 +402,7 @@ __global__ void __launch_bounds__(160, TileCfg<DH>::CTAS)
                         tmem_ld_wait(sv);
 #pragma unroll
                         for (int i = 0; i < 32; ++i)
-                            if (half[q] >> i & 1) top = fmaxf(top, __uint_as_float(sv[i] ^ flip) * c);
+                            if (half[q] >> i & 1) top = fmaxf(top, __uint_as_float(sv[i]) * c);
                     }
                     const float now = low ? fmaxf(m, top) : m;
                     const float f = now == m ? 1.f : ex2_approx(m - now);
@@ -400,17 +430,16 @@ __global__ void __launch_bounds__(160, TileCfg<DH>::CTAS)
                 if (lane == 0) mbar_arrive(bar_p);
             }
             if (!ok) break;
+            if (t + gridDim.x < p.ntiles) next = tile_at(p, t + gridDim.x);  // while the last product runs
             if (x.nkv > 0) {
                 ok = __all_sync(0xffffffffu, mbar_wait(bar_o, tiles & 1, p.err));
                 if (!ok) break;
                 ++tiles;
                 tc_fence_after();
             }
-            const int h = x.h0 + rh;
-            const float gate = valid && a.gates ? __ldg(a.gates + ((int64_t)x.s * a.Nq + token) * a.Hq + h) : 1.f;
-            const float f = gate / l;
+            const float f = sees ? gate / l : 0.f;
             T* out = (T*)a.out + (int64_t)x.s * a.o_seq + (int64_t)token * a.o_tok + (int64_t)h * a.o_head;
-            bool bad = false;
+            float odd = 0.f;  // NaN once a value of this row is not finite
 #pragma unroll
             for (int q = 0; q < 2 * DH; ++q) {
                 if (32 * q >= a.D) break;
@@ -427,7 +456,7 @@ __global__ void __launch_bounds__(160, TileCfg<DH>::CTAS)
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
                             v[e] = sees ? __uint_as_float(ov[i + e]) * f : 0.f;
-                            bad |= !isfinite(v[e]);
+                            odd = fmaf(v[e], 0.f, odd);
                         }
                         *reinterpret_cast<uint4*>(out + 32 * q + i) =
                             make_uint4(pack2(v[0], v[1], (T*)nullptr), pack2(v[2], v[3], (T*)nullptr),
@@ -437,7 +466,7 @@ __global__ void __launch_bounds__(160, TileCfg<DH>::CTAS)
                 __syncwarp();
             }
             tc_fence_before();  // O read before the next tile's first product overwrites it (behind this warp's next P)
-            for (uint32_t rows = __ballot_sync(0xffffffffu, bad); rows; rows &= rows - 1) {
+            for (uint32_t rows = __ballot_sync(0xffffffffu, odd != 0.f); rows; rows &= rows - 1) {
                 const int q = 32 * warp + __ffs(rows) - 1, qt = (int)p.by_pack.div(q);
                 attend_row<T, false, false>(a, x.s, x.tok0 + qt, x.h0 + q - qt * p.pack, x.n, x.m);
             }
