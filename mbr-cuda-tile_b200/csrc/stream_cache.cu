@@ -125,6 +125,104 @@ __global__ void __launch_bounds__(256) cache_rows_kernel(const RowArgs a) {
     }
 }
 
+// Vector form: 8 channels a lane (16-byte rows, dim_head 32, 64 or 128 for codes,
+// any multiple of 8 otherwise).  Key and value rows of four tokens of a head lie
+// next to each other in the cache, so a warp's rows are neighbouring tokens first.
+// The group's minimum and maximum are two shuffle steps (4 lanes a group).
+template <typename T, bool Q4, bool READ>
+__global__ void __launch_bounds__(256) cache_vec_kernel(const RowArgs a, int lanes_log2) {
+    const int D = a.c.dim_head, lanes = 1 << lanes_log2, sub = threadIdx.x & (lanes - 1);
+    const int64_t quads = (a.tokens + 3) >> 2;  // of tokens
+    const int64_t n = a.c.seqs * quads * a.c.kv_heads * 4;
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> lanes_log2;
+    // row i: token 4 * quad + i % 4, then head, then quad, then sequence (threads past the end stay for the shuffles)
+    const int64_t j = i >> 2, hq = j / a.c.kv_heads;
+    const int64_t s = min(hq / quads, a.c.seqs - 1);
+    Row w;
+    w.h = (int)(j - hq * a.c.kv_heads);
+    w.s = s;
+    w.t = (hq - (hq / quads) * quads) * 4 + (i & 3);
+    const bool real = i < n && w.t < a.tokens;
+    const int64_t cnt = a.count ? min((int64_t)max(a.count[s], 0), a.tokens) : a.tokens;
+    const int64_t p0 = a.pos[s], p = p0 + w.t, last = p0 + cnt - 1;
+    w.held = real && w.t < cnt && p >= 0 && p <= INT32_MAX && (p < a.c.sinks || p > last - a.c.ring);
+    const int64_t slots = (int64_t)a.c.sinks + a.c.ring;
+    w.slot_row = (w.s * a.c.kv_heads + w.h) * slots + (w.held ? slot_of((int)p, a.c.sinks, a.c.ring) : 0);
+    const int d0 = sub * 8;
+    const bool in = real && d0 < D;
+    T* x[2] = {const_cast<T*>(at<T>(a.k, w)) + d0, const_cast<T*>(at<T>(a.v, w)) + d0};
+    void* data[2] = {a.c.k, a.c.v};
+    T* scale[2] = {(T*)a.c.k_scale, (T*)a.c.v_scale};
+    constexpr int W = sizeof(T) / 2;  // 16-byte pieces of 8 elements
+    uint4 raw[2][W];
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+        if constexpr (READ && Q4) {
+            uint32_t codes = 0, sm = 0;
+            if (in && w.held) {
+                codes = *reinterpret_cast<const uint32_t*>((uint8_t*)data[kv] + w.slot_row * (D / 2) + sub * 4);
+                sm = *reinterpret_cast<const uint32_t*>(scale[kv] + (w.slot_row * (D / kGroup) + sub / 4) * 2);
+            }
+            const T* f = reinterpret_cast<const T*>(&sm);
+            T* e = reinterpret_cast<T*>(raw[kv]);
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+                e[c] = w.held ? code_value<T>((codes >> (4 * c)) & 15, to_f32<T>(f[0]), to_f32<T>(f[1])) : from_f32<T>(0.f);
+        } else {
+            const uint4* src = reinterpret_cast<const uint4*>(READ ? (T*)data[kv] + w.slot_row * D + d0 : x[kv]);
+#pragma unroll
+            for (int c = 0; c < W; ++c) raw[kv][c] = in && w.held ? __ldg(src + c) : make_uint4(0u, 0u, 0u, 0u);
+        }
+    }
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+        if constexpr (!READ && Q4) {
+            const T* e = reinterpret_cast<const T*>(raw[kv]);
+            float v[8], lo = INFINITY, hi = -INFINITY;
+            bool ok = true;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                v[c] = to_f32<T>(e[c]);
+                lo = fminf(lo, v[c]), hi = fmaxf(hi, v[c]);
+                ok = ok && isfinite(v[c]);
+            }
+#pragma unroll
+            for (int o = 1; o < 4; o <<= 1) {
+                lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+                hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+                ok = __shfl_xor_sync(0xffffffffu, (int)ok, o) && ok;
+            }
+            ok = ok && isfinite(hi - lo);
+            const T sT = from_f32<T>(__fmul_rn(hi - lo, 1.f / 15.f));
+            const float st = to_f32<T>(sT);
+            const T mT = from_f32<T>(__fadd_rn(lo, 8.f * st));
+            const float m = to_f32<T>(mT), inv = st > 0.f ? __frcp_rn(st) : 0.f;
+            uint32_t codes = 0;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                const float q = rintf(__fmul_rn(__fadd_rn(v[c], -m), inv)) + 8.f;
+                codes |= (uint32_t)(int)fminf(fmaxf(q, 0.f), 15.f) << (4 * c);
+            }
+            if (in && w.held) {
+                *reinterpret_cast<uint32_t*>((uint8_t*)data[kv] + w.slot_row * (D / 2) + sub * 4) = codes;
+                if ((sub & 3) == 0) {
+                    union {
+                        T f[2];
+                        uint32_t w32;
+                    } sm;
+                    sm.f[0] = ok ? sT : from_f32<T>(NAN);
+                    sm.f[1] = ok ? mT : from_f32<T>(NAN);
+                    *reinterpret_cast<uint32_t*>(scale[kv] + (w.slot_row * (D / kGroup) + sub / 4) * 2) = sm.w32;
+                }
+            }
+        } else if (READ ? in : in && w.held) {
+            uint4* dst = reinterpret_cast<uint4*>(READ ? x[kv] : (T*)data[kv] + w.slot_row * D + d0);
+#pragma unroll
+            for (int c = 0; c < W; ++c) dst[c] = raw[kv][c];
+        }
+    }
+}
+
 template <bool READ>
 void run(const mbr_kv_cache& c, const mbr_view& k, const mbr_view& v, const int32_t* pos, const int32_t* count,
          int64_t tokens, cudaStream_t st) {
@@ -135,6 +233,24 @@ void run(const mbr_kv_cache& c, const mbr_view& k, const mbr_view& v, const int3
     MBR_CHECK(tokens < (1 << 30) && c.seqs <= ((int64_t)1 << 50) / tokens / c.kv_heads, "kv cache: too many rows");
     RowArgs a{c, k, v, pos, count, tokens, c.seqs * tokens * c.kv_heads};
     const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(a.rows, 8), 148 * 64);
+    const int es = (int)dtype_bytes(c.dtype);
+    if (rows_aligned16(k, es) && rows_aligned16(v, es)) {
+        int lanes_log2 = 0;
+        while ((8 << lanes_log2) < c.dim_head) ++lanes_log2;
+        const int64_t rows = c.seqs * ((tokens + 3) >> 2) * c.kv_heads * 4;
+        const int64_t blocks = ceil_div(rows << lanes_log2, 256);
+        MBR_CHECK(blocks <= INT32_MAX, "kv cache: too many rows");
+        MBR_DISPATCH_DTYPE(c.dtype, T, {
+            if constexpr (std::is_same_v<T, float>) {
+                cache_vec_kernel<T, false, READ><<<(unsigned)blocks, 256, 0, st>>>(a, lanes_log2);
+            } else {
+                if (q4) cache_vec_kernel<T, true, READ><<<(unsigned)blocks, 256, 0, st>>>(a, lanes_log2);
+                else cache_vec_kernel<T, false, READ><<<(unsigned)blocks, 256, 0, st>>>(a, lanes_log2);
+            }
+        });
+        MBR_CUDA(cudaGetLastError());
+        return;
+    }
     MBR_DISPATCH_DTYPE(c.dtype, T, {
         if constexpr (std::is_same_v<T, float>) {
             cache_rows_kernel<T, false, READ><<<grid, 256, 0, st>>>(a);

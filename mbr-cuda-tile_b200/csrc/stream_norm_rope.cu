@@ -95,6 +95,98 @@ __global__ void __launch_bounds__(256) norm_rope_any_kernel(const NormRopeArgs a
     }
 }
 
+// Vector form: a head is LANES lanes x 16 bytes (dim_head a multiple of a lane's
+// elements, rows on 16-byte boundaries, every section a multiple of a lane's
+// pairs).  A warp takes one token: its lanes hold the token's (cos, sin) and
+// gains once and walk its heads 32 / LANES x UNROLL at a time, all loads of a
+// step in flight before the first is used.
+template <typename T, int LANES, int UNROLL>
+__global__ void __launch_bounds__(256) norm_rope_vec_kernel(const NormRopeArgs a) {
+    constexpr int E = 16 / sizeof(T);  // elements a lane
+    const int lane = threadIdx.x & 31, sub = lane % LANES, grp = lane / LANES;
+    constexpr int GROUPS = 32 / LANES;
+    const bool in = sub * E < a.D;  // lanes past the head size hold zeros
+    const int64_t tok = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (tok >= a.ntok) return;
+    const int64_t s = tok / a.tokens, t = tok - s * a.tokens;
+    const T* q0 = (const T*)a.q + s * a.q_seq + t * a.q_tok + sub * E;
+    const T* k0 = (const T*)a.k + s * a.k_seq + t * a.k_tok + sub * E;
+    T* qo0 = (T*)a.qo + s * a.qo_seq + t * a.qo_tok + sub * E;
+    T* ko0 = (T*)a.ko + s * a.ko_seq + t * a.ko_tok + sub * E;
+    float cs[E / 2], sn[E / 2];
+    const int i0 = sub * E / 2;
+    const bool turned = in && i0 < a.used;
+    {
+        bool ok = false;
+        int64_t at = 0;
+        if (turned) {
+            const int p = __ldg(a.pos + tok * a.axes + axis_of(a, i0));
+            ok = p >= 0 && p < a.rows;
+            at = (int64_t)p * (a.D >> 1) + i0;
+        }
+#pragma unroll
+        for (int i = 0; i < E / 2; ++i) {
+            cs[i] = ok ? __ldg(a.cs + at + i) : NAN;
+            sn[i] = ok ? __ldg(a.sn + at + i) : NAN;
+        }
+    }
+    const int HT = a.Hq + a.Hkv;
+    const float inv_d = 1.f / (float)a.D;
+    for (int h0 = grp; h0 < HT; h0 += GROUPS * UNROLL) {
+        uint4 raw[UNROLL];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const int h = h0 + u * GROUPS;
+            raw[u] = make_uint4(0u, 0u, 0u, 0u);
+            if (h < HT && in)
+                raw[u] = *reinterpret_cast<const uint4*>(h < a.Hq ? q0 + h * a.q_head : k0 + (h - a.Hq) * a.k_head);
+        }
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const int h = h0 + u * GROUPS;
+            if (u > 0 && h - grp >= HT) break;  // no group has a head left (warp-uniform)
+            const T* x = reinterpret_cast<const T*>(&raw[u]);
+            float v[E], ss = 0.f;
+#pragma unroll
+            for (int i = 0; i < E; ++i) v[i] = to_f32<T>(x[i]), ss += v[i] * v[i];
+#pragma unroll
+            for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            const float r = rsqrtf(ss * inv_d + a.eps);
+            const float* g = h < a.Hq ? a.gq : a.gk;
+            union {
+                T e[E];
+                uint4 w;
+            } y;
+#pragma unroll
+            for (int i = 0; i < E; i += 2) {
+                const float y0 = v[i] * r * (g && in ? __ldg(g + sub * E + i) : 1.f);
+                const float y1 = v[i + 1] * r * (g && in ? __ldg(g + sub * E + i + 1) : 1.f);
+                y.e[i] = from_f32<T>(turned ? y0 * cs[i / 2] - y1 * sn[i / 2] : y0);
+                y.e[i + 1] = from_f32<T>(turned ? y0 * sn[i / 2] + y1 * cs[i / 2] : y1);
+            }
+            if (h < HT && in)
+                *reinterpret_cast<uint4*>(h < a.Hq ? qo0 + h * a.qo_head : ko0 + (h - a.Hq) * a.ko_head) = y.w;
+        }
+    }
+}
+
+// Launches the vector form if the call fits it.
+template <typename T>
+bool launch_vec(const NormRopeArgs& a, bool aligned, cudaStream_t st) {
+    constexpr int E = 16 / sizeof(T);
+    bool sections = a.used % (E / 2) == 0;
+    for (int i = 0; i < 3; ++i) sections = sections && (a.end[i] == INT32_MAX || a.end[i] % (E / 2) == 0);
+    const int lanes = a.D / E;
+    const int64_t grid = ceil_div(a.ntok, 8);
+    if (!aligned || a.D % E != 0 || !sections || lanes > 32 || grid > INT32_MAX) return false;
+    const unsigned n = (unsigned)grid;
+    if (lanes <= 4) norm_rope_vec_kernel<T, 4, 2><<<n, 256, 0, st>>>(a);
+    else if (lanes <= 8) norm_rope_vec_kernel<T, 8, 4><<<n, 256, 0, st>>>(a);
+    else if (lanes <= 16) norm_rope_vec_kernel<T, 16, 4><<<n, 256, 0, st>>>(a);
+    else norm_rope_vec_kernel<T, 32, 4><<<n, 256, 0, st>>>(a);
+    return true;
+}
+
 }  // namespace
 
 void qk_norm_rope(const mbr_view& q, const mbr_view& k, const mbr_view& qo, const mbr_view& ko, int64_t seqs,
@@ -131,7 +223,12 @@ void qk_norm_rope(const mbr_view& q, const mbr_view& k, const mbr_view& qo, cons
     a.rows = table_rows, a.pos = pos, a.axes = axes;
     const int64_t warps = a.ntok * (Hq + Hkv);
     const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(warps, 8), 148 * 64);
-    MBR_DISPATCH_DTYPE(dtype, T, { norm_rope_any_kernel<T><<<grid, 256, 0, st>>>(a); });
+    const int es = (int)dtype_bytes(dtype);
+    const bool aligned = (Hq == 0 || (rows_aligned16(q, es) && rows_aligned16(qo, es))) &&
+                         (Hkv == 0 || (rows_aligned16(k, es) && rows_aligned16(ko, es)));
+    MBR_DISPATCH_DTYPE(dtype, T, {
+        if (!launch_vec<T>(a, aligned, st)) norm_rope_any_kernel<T><<<grid, 256, 0, st>>>(a);
+    });
     MBR_CUDA(cudaGetLastError());
 }
 
