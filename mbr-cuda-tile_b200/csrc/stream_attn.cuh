@@ -7,22 +7,6 @@
 namespace mbr {
 namespace streamops {
 
-// Division of 31-bit numbers by a divisor fixed for a launch: with l = ceil(log2
-// d) and mul = ceil(2^(31 + l) / d), n mul / 2^(31 + l) exceeds n / d by less
-// than 1 / d for n < 2^31.
-struct FastDiv {
-    unsigned d = 1, mul = 0, shift = 0;
-    FastDiv() = default;
-    explicit FastDiv(unsigned n) : d(n) {
-        if (n < 2) return;
-        unsigned l = 1;
-        while ((1ull << l) < n) ++l;
-        mul = (unsigned)(((1ull << (31 + l)) + n - 1) / n);
-        shift = l - 1;
-    }
-    __device__ __forceinline__ unsigned div(unsigned n) const { return d == 1 ? n : __umulhi(n, mul) >> shift; }
-};
-
 // One call's problem.  Keys are a strided view (cached = false) or the rolling
 // cache; `len` / `q_len` give the keys and queries of each sequence.
 struct AttnArgs {

@@ -42,6 +42,7 @@ struct RowArgs {
     mbr_view k, v;
     const int32_t *pos, *count;
     int64_t tokens, rows;  // rows: seqs * tokens * kv_heads
+    FastDiv by_heads, by_quads;  // vector form
 };
 
 // The row (sequence, token, head) of index r, its position and cache row; held:
@@ -132,17 +133,16 @@ __global__ void __launch_bounds__(256) cache_rows_kernel(const RowArgs a) {
 template <typename T, bool Q4, bool READ>
 __global__ void __launch_bounds__(256) cache_vec_kernel(const RowArgs a, int lanes_log2) {
     const int D = a.c.dim_head, lanes = 1 << lanes_log2, sub = threadIdx.x & (lanes - 1);
-    const int64_t quads = (a.tokens + 3) >> 2;  // of tokens
-    const int64_t n = a.c.seqs * quads * a.c.kv_heads * 4;
-    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> lanes_log2;
     // row i: token 4 * quad + i % 4, then head, then quad, then sequence (threads past the end stay for the shuffles)
-    const int64_t j = i >> 2, hq = j / a.c.kv_heads;
-    const int64_t s = min(hq / quads, a.c.seqs - 1);
+    const unsigned i = (blockIdx.x * 256 + threadIdx.x) >> lanes_log2, j = i >> 2;
+    const unsigned hq = a.by_heads.div(j);
+    const unsigned sq = a.by_quads.div(hq);
+    const int64_t s = min((int64_t)sq, a.c.seqs - 1);
     Row w;
     w.h = (int)(j - hq * a.c.kv_heads);
     w.s = s;
-    w.t = (hq - (hq / quads) * quads) * 4 + (i & 3);
-    const bool real = i < n && w.t < a.tokens;
+    w.t = (int64_t)(hq - sq * a.by_quads.d) * 4 + (i & 3);
+    const bool real = sq < a.c.seqs && w.t < a.tokens;
     const int64_t cnt = a.count ? min((int64_t)max(a.count[s], 0), a.tokens) : a.tokens;
     const int64_t p0 = a.pos[s], p = p0 + w.t, last = p0 + cnt - 1;
     w.held = real && w.t < cnt && p >= 0 && p <= INT32_MAX && (p < a.c.sinks || p > last - a.c.ring);
@@ -231,15 +231,15 @@ void run(const mbr_kv_cache& c, const mbr_view& k, const mbr_view& v, const int3
     if (c.seqs == 0 || c.kv_heads == 0 || tokens == 0) return;
     MBR_CHECK(k.data && v.data && pos, "kv cache: null buffer");
     MBR_CHECK(tokens < (1 << 30) && c.seqs <= ((int64_t)1 << 50) / tokens / c.kv_heads, "kv cache: too many rows");
-    RowArgs a{c, k, v, pos, count, tokens, c.seqs * tokens * c.kv_heads};
+    RowArgs a{c, k, v, pos, count, tokens, c.seqs * tokens * c.kv_heads, {}, {}};
     const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(a.rows, 8), 148 * 64);
     const int es = (int)dtype_bytes(c.dtype);
-    if (rows_aligned16(k, es) && rows_aligned16(v, es)) {
-        int lanes_log2 = 0;
-        while ((8 << lanes_log2) < c.dim_head) ++lanes_log2;
-        const int64_t rows = c.seqs * ((tokens + 3) >> 2) * c.kv_heads * 4;
-        const int64_t blocks = ceil_div(rows << lanes_log2, 256);
-        MBR_CHECK(blocks <= INT32_MAX, "kv cache: too many rows");
+    int lanes_log2 = 0;
+    while ((8 << lanes_log2) < c.dim_head) ++lanes_log2;
+    const int64_t quads = (tokens + 3) >> 2, threads = (c.seqs * quads * c.kv_heads * 4) << lanes_log2;
+    if (rows_aligned16(k, es) && rows_aligned16(v, es) && threads < (1ll << 31) - 256) {
+        a.by_heads = FastDiv((unsigned)c.kv_heads), a.by_quads = FastDiv((unsigned)quads);
+        const int64_t blocks = ceil_div(threads, 256);
         MBR_DISPATCH_DTYPE(c.dtype, T, {
             if constexpr (std::is_same_v<T, float>) {
                 cache_vec_kernel<T, false, READ><<<(unsigned)blocks, 256, 0, st>>>(a, lanes_log2);

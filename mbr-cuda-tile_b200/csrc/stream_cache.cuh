@@ -8,6 +8,22 @@
 namespace mbr {
 namespace streamops {
 
+// Division of 31-bit numbers by a divisor fixed for a launch: with l = ceil(log2
+// d) and mul = ceil(2^(31 + l) / d), n mul / 2^(31 + l) exceeds n / d by less
+// than 1 / d for n < 2^31.
+struct FastDiv {
+    unsigned d = 1, mul = 0, shift = 0;
+    FastDiv() = default;
+    explicit FastDiv(unsigned n) : d(n) {
+        if (n < 2) return;
+        unsigned l = 1;
+        while ((1ull << l) < n) ++l;
+        mul = (unsigned)(((1ull << (31 + l)) + n - 1) / n);
+        shift = l - 1;
+    }
+    __device__ __forceinline__ unsigned div(unsigned n) const { return d == 1 ? n : __umulhi(n, mul) >> shift; }
+};
+
 constexpr int kGroup = 32;  // channels that share a step and an offset in a 4-bit cache
 
 // Slot of position p >= 0.

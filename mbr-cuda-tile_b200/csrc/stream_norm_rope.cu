@@ -9,7 +9,7 @@
 #include <algorithm>
 
 #include "common.cuh"
-#include "stream_ops.h"
+#include "stream_cache.cuh"
 
 namespace mbr {
 namespace streamops {
@@ -31,6 +31,7 @@ struct NormRopeArgs {
     int axes;
     int end[4];  // pair index at which axis a's section ends (INT_MAX past the last)
     int used;    // pairs turned
+    FastDiv by_tokens, by_chunks;  // vector form: tokens of a sequence, steps of a token
 };
 
 // Axis of pair i (i < used).
@@ -97,79 +98,144 @@ __global__ void __launch_bounds__(256) norm_rope_any_kernel(const NormRopeArgs a
 
 // Vector form: a head is LANES lanes x 16 bytes (dim_head a multiple of a lane's
 // elements, rows on 16-byte boundaries, every section a multiple of a lane's
-// pairs).  A warp takes one token: its lanes hold the token's (cos, sin) and
-// gains once and walk its heads 32 / LANES x UNROLL at a time, all loads of a
-// step in flight before the first is used.
-template <typename T, int LANES, int UNROLL>
-__global__ void __launch_bounds__(256) norm_rope_vec_kernel(const NormRopeArgs a) {
+// pairs).  A step is 32 / LANES x UNROLL heads of one token; a warp walks steps
+// with the next step's loads (heads, then angles) in flight while it works on
+// one.  The gains lie in shared memory: in registers they would halve the warps.
+// WHOLE: every pair is turned.
+template <typename T, int LANES, int UNROLL, bool WHOLE>
+__global__ void __launch_bounds__(256, 3) norm_rope_vec_kernel(const NormRopeArgs a) {
     constexpr int E = 16 / sizeof(T);  // elements a lane
-    const int lane = threadIdx.x & 31, sub = lane % LANES, grp = lane / LANES;
     constexpr int GROUPS = 32 / LANES;
+    const int lane = threadIdx.x & 31, sub = lane % LANES, grp = lane / LANES;
     const bool in = sub * E < a.D;  // lanes past the head size hold zeros
-    const int64_t tok = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (tok >= a.ntok) return;
-    const int64_t s = tok / a.tokens, t = tok - s * a.tokens;
-    const T* q0 = (const T*)a.q + s * a.q_seq + t * a.q_tok + sub * E;
-    const T* k0 = (const T*)a.k + s * a.k_seq + t * a.k_tok + sub * E;
-    T* qo0 = (T*)a.qo + s * a.qo_seq + t * a.qo_tok + sub * E;
-    T* ko0 = (T*)a.ko + s * a.ko_seq + t * a.ko_tok + sub * E;
-    float cs[E / 2], sn[E / 2];
     const int i0 = sub * E / 2;
-    const bool turned = in && i0 < a.used;
-    {
-        bool ok = false;
-        int64_t at = 0;
-        if (turned) {
-            const int p = __ldg(a.pos + tok * a.axes + axis_of(a, i0));
-            ok = p >= 0 && p < a.rows;
-            at = (int64_t)p * (a.D >> 1) + i0;
-        }
-#pragma unroll
-        for (int i = 0; i < E / 2; ++i) {
-            cs[i] = ok ? __ldg(a.cs + at + i) : NAN;
-            sn[i] = ok ? __ldg(a.sn + at + i) : NAN;
-        }
-    }
-    const int HT = a.Hq + a.Hkv;
+    const bool turned = in && (WHOLE || i0 < a.used);
+    const int axis = turned ? axis_of(a, i0) : 0, HT = a.Hq + a.Hkv;
     const float inv_d = 1.f / (float)a.D;
-    for (int h0 = grp; h0 < HT; h0 += GROUPS * UNROLL) {
+    __shared__ float gain[2][LANES * E];
+    struct Step {
         uint4 raw[UNROLL];
+        float cs[E / 2], sn[E / 2];
+    };
+    auto place = [&](unsigned step, unsigned& s, unsigned& t, int& h0) {
+        const unsigned tok = a.by_chunks.div(step);
+        s = a.by_tokens.div(tok);
+        t = tok - s * a.by_tokens.d;
+        h0 = (int)(step - tok * a.by_chunks.d) * GROUPS * UNROLL + grp;
+        return tok;
+    };
+    auto load = [&](Step& x, unsigned step) {
+        unsigned s, t;
+        int h0;
+        const unsigned tok = place(step, s, t, h0);
+        const int p = turned ? __ldg(a.pos + (int64_t)tok * a.axes + axis) : -1;
+        const T* q0 = (const T*)a.q + (int64_t)s * a.q_seq + t * a.q_tok + sub * E;
+        const T* k0 = (const T*)a.k + (int64_t)s * a.k_seq + t * a.k_tok + sub * E;
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
             const int h = h0 + u * GROUPS;
-            raw[u] = make_uint4(0u, 0u, 0u, 0u);
+            x.raw[u] = make_uint4(0u, 0u, 0u, 0u);
             if (h < HT && in)
-                raw[u] = *reinterpret_cast<const uint4*>(h < a.Hq ? q0 + h * a.q_head : k0 + (h - a.Hq) * a.k_head);
+                x.raw[u] = *reinterpret_cast<const uint4*>(h < a.Hq ? q0 + h * a.q_head : k0 + (h - a.Hq) * a.k_head);
         }
+        const bool ok = p >= 0 && p < a.rows;
+        const int64_t at = ok ? (int64_t)p * (a.D >> 1) + i0 : 0;
+        // sections are multiples of a lane's pairs: its angles are one (or, in 32 bits, half a) 16-byte piece
+        if constexpr (E == 8) {
+            const float4 c = ok ? __ldg(reinterpret_cast<const float4*>(a.cs + at)) : make_float4(NAN, NAN, NAN, NAN);
+            const float4 n = ok ? __ldg(reinterpret_cast<const float4*>(a.sn + at)) : make_float4(NAN, NAN, NAN, NAN);
+            x.cs[0] = c.x, x.cs[1] = c.y, x.cs[2] = c.z, x.cs[3] = c.w;
+            x.sn[0] = n.x, x.sn[1] = n.y, x.sn[2] = n.z, x.sn[3] = n.w;
+        } else {
+            const float2 c = ok ? __ldg(reinterpret_cast<const float2*>(a.cs + at)) : make_float2(NAN, NAN);
+            const float2 n = ok ? __ldg(reinterpret_cast<const float2*>(a.sn + at)) : make_float2(NAN, NAN);
+            x.cs[0] = c.x, x.cs[1] = c.y;
+            x.sn[0] = n.x, x.sn[1] = n.y;
+        }
+    };
+    const unsigned steps = (unsigned)a.ntok * a.by_chunks.d, stride = gridDim.x * 8;
+    unsigned step = blockIdx.x * 8 + (threadIdx.x >> 5);
+    Step x;
+    if (step < steps) load(x, step);
+    for (int i = threadIdx.x; i < 2 * LANES * E; i += 256) {
+        const int d = i % (LANES * E);
+        const float* g = i < LANES * E ? a.gq : a.gk;
+        gain[i / (LANES * E)][d] = g && d < a.D ? __ldg(g + d) : 1.f;
+    }
+    __syncthreads();
+    if (step >= steps) return;
+    for (;;) {
+        const bool more = step + stride < steps;
+        Step y;
+        if (more) load(y, step + stride);
+        unsigned s, t;
+        int h0;
+        place(step, s, t, h0);
+        T* qo0 = (T*)a.qo + (int64_t)s * a.qo_seq + t * a.qo_tok + sub * E;
+        T* ko0 = (T*)a.ko + (int64_t)s * a.ko_seq + t * a.ko_tok + sub * E;
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
             const int h = h0 + u * GROUPS;
-            if (u > 0 && h - grp >= HT) break;  // no group has a head left (warp-uniform)
-            const T* x = reinterpret_cast<const T*>(&raw[u]);
-            float v[E], ss = 0.f;
+            // pairs (2i, 2i + 1) throughout, two fp32 operations an instruction
+            const typename PairOf<T>::type* e = reinterpret_cast<const typename PairOf<T>::type*>(&x.raw[u]);
+            float2 v[E / 2], sq = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int i = 0; i < E; ++i) v[i] = to_f32<T>(x[i]), ss += v[i] * v[i];
+            for (int i = 0; i < E / 2; ++i) v[i] = pair_to_f32<T>(e[i]), sq = __ffma2_rn(v[i], v[i], sq);
+            float ss = sq.x + sq.y;
 #pragma unroll
             for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
             const float r = rsqrtf(ss * inv_d + a.eps);
-            const float* g = h < a.Hq ? a.gq : a.gk;
+            const bool isq = h < a.Hq;
+            const float2* g = reinterpret_cast<const float2*>(&gain[isq ? 0 : 1][sub * E]);
             union {
                 T e[E];
                 uint4 w;
-            } y;
+            } z;
 #pragma unroll
-            for (int i = 0; i < E; i += 2) {
-                const float y0 = v[i] * r * (g && in ? __ldg(g + sub * E + i) : 1.f);
-                const float y1 = v[i + 1] * r * (g && in ? __ldg(g + sub * E + i + 1) : 1.f);
-                y.e[i] = from_f32<T>(turned ? y0 * cs[i / 2] - y1 * sn[i / 2] : y0);
-                y.e[i + 1] = from_f32<T>(turned ? y0 * sn[i / 2] + y1 * cs[i / 2] : y1);
+            for (int i = 0; i < E / 2; ++i) {
+                const float2 y = __fmul2_rn(__fmul2_rn(v[i], make_float2(r, r)), g[i]);
+                const float2 n = __ffma2_rn(y, make_float2(x.cs[i], x.cs[i]),
+                                            __fmul2_rn(make_float2(y.y, y.x), make_float2(-x.sn[i], x.sn[i])));
+                store_pair<T>(&z.e[2 * i], WHOLE || turned ? n : y);
             }
             if (h < HT && in)
-                *reinterpret_cast<uint4*>(h < a.Hq ? qo0 + h * a.qo_head : ko0 + (h - a.Hq) * a.ko_head) = y.w;
+                *reinterpret_cast<uint4*>(isq ? qo0 + h * a.qo_head : ko0 + (h - a.Hq) * a.ko_head) = z.w;
         }
+        if (!more) break;
+        x = y;
+        step += stride;
     }
 }
 
+template <typename T, int LANES, int UNROLL, bool WHOLE>
+void launch_steps(NormRopeArgs a, cudaStream_t st) {
+    constexpr int heads = 32 / LANES * UNROLL;
+    const int64_t chunks = ceil_div(a.Hq + a.Hkv, heads);
+    a.by_tokens = FastDiv((unsigned)a.tokens), a.by_chunks = FastDiv((unsigned)chunks);
+    auto kern = norm_rope_vec_kernel<T, LANES, UNROLL, WHOLE>;
+    static int wave[kMaxStreamDevices] = {};  // CTAs that fit the device at once
+    const int dev = stream_device();
+    if (!wave[dev]) {
+        int per = 0, sms = 0;
+        MBR_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kern, 256, 0));
+        MBR_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+        wave[dev] = std::max(1, per * sms);
+    }
+    kern<<<(unsigned)std::min<int64_t>(ceil_div(a.ntok * chunks, 8), wave[dev]), 256, 0, st>>>(a);
+}
+
+// With few tokens a step is one head a lane group (more warps share the latency),
+// otherwise four (more loads in flight a warp).
+template <typename T, int LANES, bool WHOLE>
+void launch_unrolled(const NormRopeArgs& a, cudaStream_t st) {
+    if (a.ntok * (a.Hq + a.Hkv) <= 148 * 8 * 32 / LANES) launch_steps<T, LANES, 1, WHOLE>(a, st);
+    else launch_steps<T, LANES, 4, WHOLE>(a, st);
+}
+template <typename T, int LANES>
+void launch_lanes(const NormRopeArgs& a, cudaStream_t st) {
+    if (2 * a.used == a.D) launch_unrolled<T, LANES, true>(a, st);
+    else launch_unrolled<T, LANES, false>(a, st);
+}
 // Launches the vector form if the call fits it.
 template <typename T>
 bool launch_vec(const NormRopeArgs& a, bool aligned, cudaStream_t st) {
@@ -177,13 +243,11 @@ bool launch_vec(const NormRopeArgs& a, bool aligned, cudaStream_t st) {
     bool sections = a.used % (E / 2) == 0;
     for (int i = 0; i < 3; ++i) sections = sections && (a.end[i] == INT32_MAX || a.end[i] % (E / 2) == 0);
     const int lanes = a.D / E;
-    const int64_t grid = ceil_div(a.ntok, 8);
-    if (!aligned || a.D % E != 0 || !sections || lanes > 32 || grid > INT32_MAX) return false;
-    const unsigned n = (unsigned)grid;
-    if (lanes <= 4) norm_rope_vec_kernel<T, 4, 2><<<n, 256, 0, st>>>(a);
-    else if (lanes <= 8) norm_rope_vec_kernel<T, 8, 4><<<n, 256, 0, st>>>(a);
-    else if (lanes <= 16) norm_rope_vec_kernel<T, 16, 4><<<n, 256, 0, st>>>(a);
-    else norm_rope_vec_kernel<T, 32, 4><<<n, 256, 0, st>>>(a);
+    if (!aligned || a.D % E != 0 || !sections || lanes > 32 || a.ntok * (a.Hq + a.Hkv) >= (1ll << 30)) return false;
+    if (lanes <= 4) launch_lanes<T, 4>(a, st);
+    else if (lanes <= 8) launch_lanes<T, 8>(a, st);
+    else if (lanes <= 16) launch_lanes<T, 16>(a, st);
+    else launch_lanes<T, 32>(a, st);
     return true;
 }
 
@@ -225,7 +289,8 @@ void qk_norm_rope(const mbr_view& q, const mbr_view& k, const mbr_view& qo, cons
     const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(warps, 8), 148 * 64);
     const int es = (int)dtype_bytes(dtype);
     const bool aligned = (Hq == 0 || (rows_aligned16(q, es) && rows_aligned16(qo, es))) &&
-                         (Hkv == 0 || (rows_aligned16(k, es) && rows_aligned16(ko, es)));
+                         (Hkv == 0 || (rows_aligned16(k, es) && rows_aligned16(ko, es))) &&
+                         (((uintptr_t)cs | (uintptr_t)sn) & 15) == 0;
     MBR_DISPATCH_DTYPE(dtype, T, {
         if (!launch_vec<T>(a, aligned, st)) norm_rope_any_kernel<T><<<grid, 256, 0, st>>>(a);
     });
