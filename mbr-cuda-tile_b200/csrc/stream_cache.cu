@@ -126,99 +126,125 @@ __global__ void __launch_bounds__(256) cache_rows_kernel(const RowArgs a) {
     }
 }
 
-// Vector form: 8 channels a lane (16-byte rows, dim_head 32, 64 or 128 for codes,
-// any multiple of 8 otherwise).  Key and value rows of four tokens of a head lie
-// next to each other in the cache, so a warp's rows are neighbouring tokens first.
-// The group's minimum and maximum are two shuffle steps (4 lanes a group).
+// Vector form: 8 channels a lane (rows on 16-byte boundaries).  A lane group takes
+// four neighbouring tokens of one head, whose cache rows lie next to each other:
+// their place is worked out once, and all eight loads are in flight before the
+// first is used.  A 4-bit group's minimum and maximum are two shuffle steps
+// (4 lanes a group).
 template <typename T, bool Q4, bool READ>
 __global__ void __launch_bounds__(256) cache_vec_kernel(const RowArgs a, int lanes_log2) {
     const int D = a.c.dim_head, lanes = 1 << lanes_log2, sub = threadIdx.x & (lanes - 1);
-    // row i: token 4 * quad + i % 4, then head, then quad, then sequence (threads past the end stay for the shuffles)
-    const unsigned i = (blockIdx.x * 256 + threadIdx.x) >> lanes_log2, j = i >> 2;
-    const unsigned hq = a.by_heads.div(j);
-    const unsigned sq = a.by_quads.div(hq);
-    const int64_t s = min((int64_t)sq, a.c.seqs - 1);
-    Row w;
-    w.h = (int)(j - hq * a.c.kv_heads);
-    w.s = s;
-    w.t = (int64_t)(hq - sq * a.by_quads.d) * 4 + (i & 3);
-    const bool real = sq < a.c.seqs && w.t < a.tokens;
-    const int64_t cnt = a.count ? min((int64_t)max(a.count[s], 0), a.tokens) : a.tokens;
-    const int64_t p0 = a.pos[s], p = p0 + w.t, last = p0 + cnt - 1;
-    w.held = real && w.t < cnt && p >= 0 && p <= INT32_MAX && (p < a.c.sinks || p > last - a.c.ring);
-    const int64_t slots = (int64_t)a.c.sinks + a.c.ring;
-    w.slot_row = (w.s * a.c.kv_heads + w.h) * slots + (w.held ? slot_of((int)p, a.c.sinks, a.c.ring) : 0);
+    // group: head, then four tokens, then sequence (threads past the end stay for the shuffles)
+    const unsigned grp = (blockIdx.x * 256 + threadIdx.x) >> lanes_log2;
+    const unsigned hq = a.by_heads.div(grp), sq = a.by_quads.div(hq);
+    const int h = (int)(grp - hq * a.c.kv_heads), t0 = (int)(hq - sq * a.by_quads.d) * 4;
+    const bool real = sq < a.c.seqs;
+    const int64_t s = real ? sq : 0;
     const int d0 = sub * 8;
     const bool in = real && d0 < D;
-    T* x[2] = {const_cast<T*>(at<T>(a.k, w)) + d0, const_cast<T*>(at<T>(a.v, w)) + d0};
-    void* data[2] = {a.c.k, a.c.v};
-    T* scale[2] = {(T*)a.c.k_scale, (T*)a.c.v_scale};
-    constexpr int W = sizeof(T) / 2;  // 16-byte pieces of 8 elements
-    uint4 raw[2][W];
+    const int tokens = (int)a.tokens;
+    const int cnt = a.count ? min(max(__ldg(a.count + s), 0), tokens) : tokens;
+    const int64_t p0 = __ldg(a.pos + s), last = p0 + cnt - 1;
+    const int64_t base = (s * a.c.kv_heads + h) * ((int64_t)a.c.sinks + a.c.ring);
+    int64_t row[4];  // cache row of each token, -1: not in the cache
 #pragma unroll
-    for (int kv = 0; kv < 2; ++kv) {
-        if constexpr (READ && Q4) {
-            uint32_t codes = 0, sm = 0;
-            if (in && w.held) {
-                codes = *reinterpret_cast<const uint32_t*>((uint8_t*)data[kv] + w.slot_row * (D / 2) + sub * 4);
-                sm = *reinterpret_cast<const uint32_t*>(scale[kv] + (w.slot_row * (D / kGroup) + sub / 4) * 2);
-            }
-            const T* f = reinterpret_cast<const T*>(&sm);
-            T* e = reinterpret_cast<T*>(raw[kv]);
-#pragma unroll
-            for (int c = 0; c < 8; ++c)
-                e[c] = w.held ? code_value<T>((codes >> (4 * c)) & 15, to_f32<T>(f[0]), to_f32<T>(f[1])) : from_f32<T>(0.f);
-        } else {
-            const uint4* src = reinterpret_cast<const uint4*>(READ ? (T*)data[kv] + w.slot_row * D + d0 : x[kv]);
-#pragma unroll
-            for (int c = 0; c < W; ++c) raw[kv][c] = in && w.held ? __ldg(src + c) : make_uint4(0u, 0u, 0u, 0u);
+    for (int u = 0; u < 4; ++u) {
+        const int64_t p = p0 + t0 + u;
+        const bool held = in && t0 + u < cnt && p >= 0 && p <= INT32_MAX && (p < a.c.sinks || p > last - a.c.ring);
+        row[u] = -1;
+        if (held) {
+            // the token after a held one follows it in the ring, but for the ring's end
+            if (u > 0 && row[u - 1] >= 0 && p > a.c.sinks)
+                row[u] = row[u - 1] + 1 < base + a.c.sinks + a.c.ring ? row[u - 1] + 1 : base + a.c.sinks;
+            else
+                row[u] = base + slot_of((int)p, a.c.sinks, a.c.ring);
         }
     }
+    constexpr int W = sizeof(T) / 2;  // 16-byte pieces of 8 elements
 #pragma unroll
     for (int kv = 0; kv < 2; ++kv) {
-        if constexpr (!READ && Q4) {
-            const T* e = reinterpret_cast<const T*>(raw[kv]);
-            float v[8], lo = INFINITY, hi = -INFINITY;
-            bool ok = true;
+        const mbr_view& view = kv ? a.v : a.k;
+        T* const x0 = (T*)view.data + s * view.seq + t0 * view.token + h * view.head + d0;
+        uint8_t* const data = (uint8_t*)(kv ? a.c.v : a.c.k);
+        T* const scale = (T*)(kv ? a.c.v_scale : a.c.k_scale);
+        uint4 raw[4][W];
+        if constexpr (READ && Q4) {
+            uint32_t codes[4], sm[4];
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                v[c] = to_f32<T>(e[c]);
-                lo = fminf(lo, v[c]), hi = fmaxf(hi, v[c]);
-                ok = ok && isfinite(v[c]);
-            }
-#pragma unroll
-            for (int o = 1; o < 4; o <<= 1) {
-                lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-                hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-                ok = __shfl_xor_sync(0xffffffffu, (int)ok, o) && ok;
-            }
-            ok = ok && isfinite(hi - lo);
-            const T sT = from_f32<T>(__fmul_rn(hi - lo, 1.f / 15.f));
-            const float st = to_f32<T>(sT);
-            const T mT = from_f32<T>(__fadd_rn(lo, 8.f * st));
-            const float m = to_f32<T>(mT), inv = st > 0.f ? __frcp_rn(st) : 0.f;
-            uint32_t codes = 0;
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                const float q = rintf(__fmul_rn(__fadd_rn(v[c], -m), inv)) + 8.f;
-                codes |= (uint32_t)(int)fminf(fmaxf(q, 0.f), 15.f) << (4 * c);
-            }
-            if (in && w.held) {
-                *reinterpret_cast<uint32_t*>((uint8_t*)data[kv] + w.slot_row * (D / 2) + sub * 4) = codes;
-                if ((sub & 3) == 0) {
-                    union {
-                        T f[2];
-                        uint32_t w32;
-                    } sm;
-                    sm.f[0] = ok ? sT : from_f32<T>(NAN);
-                    sm.f[1] = ok ? mT : from_f32<T>(NAN);
-                    *reinterpret_cast<uint32_t*>(scale[kv] + (w.slot_row * (D / kGroup) + sub / 4) * 2) = sm.w32;
+            for (int u = 0; u < 4; ++u) {
+                codes[u] = sm[u] = 0;
+                if (row[u] >= 0) {
+                    codes[u] = *reinterpret_cast<const uint32_t*>(data + row[u] * (D / 2) + sub * 4);
+                    sm[u] = *reinterpret_cast<const uint32_t*>(scale + (row[u] * (D / kGroup) + sub / 4) * 2);
                 }
             }
-        } else if (READ ? in : in && w.held) {
-            uint4* dst = reinterpret_cast<uint4*>(READ ? x[kv] : (T*)data[kv] + w.slot_row * D + d0);
 #pragma unroll
-            for (int c = 0; c < W; ++c) dst[c] = raw[kv][c];
+            for (int u = 0; u < 4; ++u) {  // a token that is not held has step and offset 0: zeros
+                const T* f = reinterpret_cast<const T*>(&sm[u]);
+                T* e = reinterpret_cast<T*>(raw[u]);
+                const float st = to_f32<T>(f[0]), m = to_f32<T>(f[1]);
+#pragma unroll
+                for (int c = 0; c < 8; c += 2)
+                    store_pair<T>(e + c, make_float2(m + st * (float)((int)((codes[u] >> (4 * c)) & 15) - 8),
+                                                     m + st * (float)((int)((codes[u] >> (4 * c + 4)) & 15) - 8)));
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const uint4* src = reinterpret_cast<const uint4*>(READ ? (const T*)data + row[u] * D + d0 : x0 + u * view.token);
+#pragma unroll
+                for (int c = 0; c < W; ++c) raw[u][c] = row[u] >= 0 ? src[c] : make_uint4(0u, 0u, 0u, 0u);
+            }
+        }
+        if constexpr (!READ && Q4) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const T* e = reinterpret_cast<const T*>(raw[u]);
+                float v[8], lo = INFINITY, hi = -INFINITY, odd = 0.f;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    v[c] = to_f32<T>(e[c]);
+                    lo = fminf(lo, v[c]), hi = fmaxf(hi, v[c]);
+                    odd = fmaf(v[c], 0.f, odd);  // NaN once a value is not finite
+                }
+#pragma unroll
+                for (int o = 1; o < 4; o <<= 1) {
+                    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+                    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+                    odd += __shfl_xor_sync(0xffffffffu, odd, o);
+                }
+                const bool ok = odd == 0.f && isfinite(hi - lo);
+                const T sT = from_f32<T>(__fmul_rn(hi - lo, 1.f / 15.f));
+                const float st = to_f32<T>(sT);
+                const T mT = from_f32<T>(__fadd_rn(lo, 8.f * st));
+                const float m = to_f32<T>(mT), inv = st > 0.f ? __frcp_rn(st) : 0.f;
+                uint32_t codes = 0;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    const float q = rintf(__fmul_rn(__fadd_rn(v[c], -m), inv)) + 8.f;
+                    codes |= (uint32_t)(int)fminf(fmaxf(q, 0.f), 15.f) << (4 * c);
+                }
+                if (row[u] >= 0) {
+                    *reinterpret_cast<uint32_t*>(data + row[u] * (D / 2) + sub * 4) = codes;
+                    if ((sub & 3) == 0) {
+                        union {
+                            T f[2];
+                            uint32_t w;
+                        } sm;
+                        sm.f[0] = ok ? sT : from_f32<T>(NAN);
+                        sm.f[1] = ok ? mT : from_f32<T>(NAN);
+                        *reinterpret_cast<uint32_t*>(scale + (row[u] * (D / kGroup) + sub / 4) * 2) = sm.w;
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (READ ? !(in && t0 + u < tokens) : row[u] < 0) continue;
+                uint4* dst = reinterpret_cast<uint4*>(READ ? x0 + u * view.token : (T*)data + row[u] * D + d0);
+#pragma unroll
+                for (int c = 0; c < W; ++c) dst[c] = raw[u][c];
+            }
         }
     }
 }
@@ -236,7 +262,7 @@ void run(const mbr_kv_cache& c, const mbr_view& k, const mbr_view& v, const int3
     const int es = (int)dtype_bytes(c.dtype);
     int lanes_log2 = 0;
     while ((8 << lanes_log2) < c.dim_head) ++lanes_log2;
-    const int64_t quads = (tokens + 3) >> 2, threads = (c.seqs * quads * c.kv_heads * 4) << lanes_log2;
+    const int64_t quads = (tokens + 3) >> 2, threads = (c.seqs * quads * c.kv_heads) << lanes_log2;
     if (rows_aligned16(k, es) && rows_aligned16(v, es) && threads < (1ll << 31) - 256) {
         a.by_heads = FastDiv((unsigned)c.kv_heads), a.by_quads = FastDiv((unsigned)quads);
         const int64_t blocks = ceil_div(threads, 256);
