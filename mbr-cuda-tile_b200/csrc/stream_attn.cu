@@ -4,6 +4,7 @@
 #include <cmath>
 
 #include "stream_attn.cuh"
+#include "stream_attn_simt.h"
 #include "stream_attn_step.h"
 #include "stream_attn_tc.h"
 
@@ -34,32 +35,20 @@ int* stream_error_word() {
 
 namespace {
 
-// One warp per row: right for every layout and type.
-template <typename T, bool CACHED, bool Q4>
+// One warp per row over an fp32 cache, whose rows no other kernel takes.
 __global__ void __launch_bounds__(256) attend_rows_kernel(const AttnArgs a) {
     const int64_t rows = a.seqs * a.Nq * a.Hq, step = (int64_t)gridDim.x * 8;
     for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += step) {
         const int64_t si = r / a.Hq, s = si / a.Nq;
         int n, m;
-        lengths<CACHED>(a, s, n, m);
-        attend_row<T, CACHED, Q4>(a, s, (int)(si - s * a.Nq), (int)(r - si * a.Hq), n, m);
+        lengths<true>(a, s, n, m);
+        attend_row<float, true, false>(a, s, (int)(si - s * a.Nq), (int)(r - si * a.Hq), n, m);
     }
 }
 
-template <bool CACHED>
-void launch_rows(const AttnArgs& a, int dtype, bool q4, cudaStream_t st) {
+void launch_rows(const AttnArgs& a, cudaStream_t st) {
     const int64_t rows = a.seqs * a.Nq * a.Hq;
-    const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(rows, 8), 148 * 64);
-    MBR_DISPATCH_DTYPE(dtype, T, {
-        if constexpr (CACHED && !std::is_same_v<T, float>) {
-            if (q4) {
-                attend_rows_kernel<T, true, true><<<grid, 256, 0, st>>>(a);
-                MBR_CUDA(cudaGetLastError());
-                return;
-            }
-        }
-        attend_rows_kernel<T, CACHED, false><<<grid, 256, 0, st>>>(a);
-    });
+    attend_rows_kernel<<<(unsigned)std::min<int64_t>(ceil_div(rows, 8), 148 * 64), 256, 0, st>>>(a);
     MBR_CUDA(cudaGetLastError());
 }
 
@@ -146,7 +135,7 @@ void window_attention(const mbr_view& q, const mbr_view& k, const mbr_view& v, c
         attend_tiles(a, dtype, st);
         return;
     }
-    launch_rows<false>(a, dtype, false, st);
+    attend_simt(a, dtype, st);
 }
 
 int64_t cache_attention_workspace(const mbr_kv_cache& c, int64_t tokens, int Hq, int left, int right) {
@@ -173,7 +162,7 @@ void cache_attention(const mbr_view& q, const mbr_kv_cache& c, const mbr_view& o
         attend_step(a, c.dtype, true, q4, pl, workspace, st);
         return;
     }
-    launch_rows<true>(a, c.dtype, q4, st);
+    launch_rows(a, st);
 }
 
 }  // namespace streamops

@@ -73,8 +73,8 @@ __device__ __forceinline__ float kv_elem(const AttnArgs& a, bool val, int64_t s,
     }
 }
 
-// The attention of one row (sequence s, query i, head h) by one warp, key after
-// key with the running maximum and sum of the softmax in fp32; lane l holds
+// The attention of one row (sequence s, query i, head h) by one warp, four keys at
+// a time with the running maximum and sum of the softmax in fp32; lane l holds
 // channels l, l + 32, ...  Keys outside the row's window are not read, so
 // nothing they hold can reach the result.  NaN scores make the row NaN.
 template <typename T, bool CACHED, bool Q4>
@@ -92,26 +92,47 @@ __device__ __noinline__ void attend_row(const AttnArgs& a, int64_t s, int i, int
         acc[c] = 0.f;
     }
     float top = -INFINITY, sum = 0.f;
+    constexpr int U = 4;  // keys at a time: their loads and shuffles overlap
     for (int pass = 0; pass < 2; ++pass) {
         const int j0 = pass ? w.lo : 0, j1 = pass ? w.hi : w.first;
-        for (int j = j0; j < j1; ++j) {
-            float dot = 0.f;
+        for (int j = j0; j < j1; j += U) {
+            float x[U], v[U][4];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const int d = lane + 32 * c;
-                if (d < a.D) dot = fmaf(qv[c], kv_elem<T, CACHED, Q4>(a, false, s, hk, j, d), dot);
+            for (int u = 0; u < U; ++u) {
+                x[u] = 0.f;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const int d = lane + 32 * c;
+                    v[u][c] = 0.f;
+                    if (d < a.D && j + u < j1) {
+                        x[u] = fmaf(qv[c], kv_elem<T, CACHED, Q4>(a, false, s, hk, j + u, d), x[u]);
+                        v[u][c] = kv_elem<T, CACHED, Q4>(a, true, s, hk, j + u, d);
+                    }
+                }
             }
-            const float x = warp_sum(dot) * a.scale;
-            // a maximum of -inf (every score so far -inf) leaves exp(-inf - -inf): such keys weigh nothing
-            const float now = fmaxf(top, x);
-            const float old = now == -INFINITY ? 1.f : expf(top - now);
-            const float e = now == -INFINITY && x == x ? 0.f : expf(x - now);
-            top = now;
-            sum = sum * old + e;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const int d = lane + 32 * c;
-                if (d < a.D) acc[c] = acc[c] * old + e * kv_elem<T, CACHED, Q4>(a, true, s, hk, j, d);
+            for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+                for (int u = 0; u < U; ++u) x[u] += __shfl_xor_sync(0xffffffffu, x[u], o);
+            float now = top;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                x[u] *= a.scale;
+                if (j + u < j1) now = fmaxf(now, x[u]);
+            }
+            // a maximum of -inf (every score so far -inf) leaves exp(-inf - -inf): such keys weigh nothing
+            const float old = now == -INFINITY ? 1.f : expf(top - now);
+            top = now;
+            sum *= old;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[c] *= old;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (j + u >= j1) break;
+                const float e = now == -INFINITY && x[u] == x[u] ? 0.f : expf(x[u] - now);
+                sum += e;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) acc[c] = fmaf(e, v[u][c], acc[c]);
             }
         }
     }

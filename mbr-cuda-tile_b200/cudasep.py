@@ -242,14 +242,33 @@ def op_attention(q, k, v, scale=0.0, gates=None, out=None, stream=None):
 
 
 # ---- streaming time-axis attention ----
+# A frame's kernels take two or three microseconds, so what these wrappers do per
+# call is kept short: each tensor is looked at once, its view packed on the spot.
 _VIEW = struct.Struct("@Pqqq")  # mbr_view
 _CACHE = struct.Struct("@PPPPqiiiiii")  # mbr_kv_cache
+_T = None  # torch and what is used of it per call, see _torch()
 
 
-def _view(t) -> bytes:
-    """mbr_view of a [seqs, tokens, heads, dim_head] tensor."""
-    a, b, c, _ = t.stride()
-    return _VIEW.pack(t.data_ptr(), a, b, c)
+class _Torch:
+    """torch's names that the streaming operators use per call."""
+
+    def __init__(self):
+        import torch
+
+        self.torch = torch
+        self.empty = torch.empty
+        self.codes = {torch.float32: FP32, torch.float16: FP16, torch.bfloat16: BF16}
+        self.f32, self.i32, self.u8 = torch.float32, torch.int32, torch.uint8
+        self.current_device = torch.cuda.current_device
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # the stream's handle without a Stream object
+        self.raw_stream = raw or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
+def _torch() -> _Torch:
+    global _T
+    if _T is None:
+        _T = _Torch()
+    return _T
 
 
 def _need(cond, msg):
@@ -257,43 +276,51 @@ def _need(cond, msg):
         raise ValueError(msg)
 
 
-def _need_rows(device, dtype, **tensors):
-    """Every tensor is [seqs, tokens, heads, dim_head] of `dtype` on `device` with its last axis contiguous."""
-    for name, t in tensors.items():
-        if t.dim() != 4 or t.dtype != dtype or t.device != device or (t.shape[3] > 1 and t.stride(3) != 1):
-            raise ValueError(f"{name} must be [seqs, tokens, heads, dim_head] of {dtype} on {device} with a contiguous "
-                             f"last axis, got {tuple(t.shape)} of {t.dtype} on {t.device}")
+def _rows(name, t, dtype, dev) -> bytes:
+    """mbr_view of a [seqs, tokens, heads, dim_head] tensor of this type on this device, last axis contiguous."""
+    st = t.stride()
+    if len(st) != 4 or t.dtype is not dtype or t.get_device() != dev or (st[3] != 1 and t.shape[3] > 1):
+        raise ValueError(f"{name} must be [seqs, tokens, heads, dim_head] of {dtype} on cuda:{dev} with a contiguous "
+                         f"last axis, got {tuple(t.shape)} of {t.dtype} on {t.device}")
+    return _VIEW.pack(t.data_ptr(), st[0], st[1], st[2])
 
 
-def _need_flat(device, dtype, shape, **tensors):
-    """Every tensor that is not None is contiguous, of this type and shape, on `device`."""
-    for name, t in tensors.items():
-        if t is not None and (t.dtype != dtype or t.device != device or tuple(t.shape) != shape
-                              or not t.is_contiguous()):
-            raise ValueError(f"{name} must be contiguous {dtype} of shape {shape} on {device}, "
-                             f"got {tuple(t.shape)} of {t.dtype} on {t.device}")
+def _flat(name, t, dtype, dev, shape):
+    """Address of a contiguous tensor of this type and shape on this device; None if there is none."""
+    if t is None:
+        return None
+    if t.dtype is not dtype or t.get_device() != dev or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous {dtype} of shape {shape} on cuda:{dev}, "
+                         f"got {tuple(t.shape)} of {t.dtype} on {t.device}")
+    return t.data_ptr()
 
 
-class _on:
-    """The device of a call's tensors is current while the call is made."""
+def _device(t) -> int:
+    dev = t.get_device()
+    _need(dev >= 0, f"tensors must be on a CUDA device, got {t.device}")
+    return dev
 
-    __slots__ = ("guard",)
 
-    def __init__(self, device):
-        import torch
+def _call(fn, dev, stream, *args):
+    """fn(*args, stream) with `dev` current; stream None is torch's current one there."""
+    T = _T
+    if stream is None:
+        stream = T.raw_stream(dev)
+    elif not isinstance(stream, int):
+        stream = stream.cuda_stream
+    if T.current_device() == dev:
+        rc = fn(*args, stream)
+    else:
+        with T.torch.cuda.device(dev):
+            rc = fn(*args, stream)
+    if rc:
+        _check(rc)
 
-        if device.type != "cuda":
-            raise ValueError(f"tensors must be on a CUDA device, got {device}")
-        same = device.index == torch.cuda.current_device()
-        self.guard = None if same else torch.cuda.device(device)
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _code(dtype) -> int:
+    code = _torch().codes.get(dtype)
+    _need(code is not None, f"dtype must be float32, float16 or bfloat16, got {dtype}")
+    return code
 
 
 def op_qk_norm_rope(q, k, gamma_q=None, gamma_k=None, cos=None, sin=None, pos=None, pairs=(), eps=1e-6, q_out=None,
@@ -302,50 +329,30 @@ def op_qk_norm_rope(q, k, gamma_q=None, gamma_k=None, cos=None, sin=None, pos=No
     (x / sqrt(mean x^2 + eps) * gamma) and rotated: pairs[a] pairs (2i, 2i+1) turn by row pos[s, t, a] of the tables
     cos, sin [rows, dim_head / 2].  pos int32 [seqs, tokens, len(pairs)].  q, k may be strided views (last axis
     contiguous); q_out / k_out may be q / k themselves."""
-    import torch
-
+    T = _torch()
+    dev, dt = _device(q), q.dtype
+    vq, vk = _rows("q", q, dt, dev), _rows("k", k, dt, dev)
     S, N, H, D = q.shape
-    dev, dt = q.device, q.dtype
-    q_out = torch.empty((S, N, H, D), dtype=dt, device=dev) if q_out is None else q_out
-    k_out = torch.empty(k.shape, dtype=dt, device=dev) if k_out is None else k_out
-    _need_rows(dev, dt, q=q, k=k, q_out=q_out, k_out=k_out)
-    _need(k.shape[0] == S and k.shape[1] == N and k.shape[3] == D, "q and k must have the same seqs, tokens, dim_head")
-    _need(q_out.shape == q.shape and k_out.shape == k.shape, "outputs must have the shapes of q and k")
-    _need_flat(dev, torch.float32, (D,), gamma_q=gamma_q, gamma_k=gamma_k)
-    axes, rows = len(pairs), 0
+    ks = k.shape
+    G = ks[2]
+    _need(ks == (S, N, G, D), "q and k must have the same seqs, tokens, dim_head")
+    if q_out is None:
+        q_out = T.empty((S, N, H, D), dtype=dt, device=q.device)
+    if k_out is None:
+        k_out = T.empty((S, N, G, D), dtype=dt, device=q.device)
+    _need(q_out.shape == q.shape and k_out.shape == ks, "outputs must have the shapes of q and k")
+    axes = len(pairs)
+    rows, c, s, p = 0, None, None, None
     if axes:
         _need(cos is not None and sin is not None and pos is not None, "cos, sin and pos are needed with pairs")
         rows = cos.shape[0]
-        _need_flat(dev, torch.float32, (rows, D // 2), cos=cos, sin=sin)
-        _need_flat(dev, torch.int32, (S, N, axes), pos=pos)
-    with _on(dev):
-        _check(lib().mbr_op_qk_norm_rope(
-            _view(q), _view(k), _view(q_out), _view(k_out), S, N, H, k.shape[2], D, _opt(gamma_q), _opt(gamma_k), eps,
-            _opt(cos), _opt(sin), rows, _opt(pos), axes, struct.pack(f"@{axes}i", *pairs), _dt(q), _stream(stream)))
+        c, s = _flat("cos", cos, T.f32, dev, (rows, D // 2)), _flat("sin", sin, T.f32, dev, (rows, D // 2))
+        p = _flat("pos", pos, T.i32, dev, (S, N, axes))
+    _call((_lib or lib()).mbr_op_qk_norm_rope, dev, stream, vq, vk, _rows("q_out", q_out, dt, dev),
+          _rows("k_out", k_out, dt, dev), S, N, H, G, D, _flat("gamma_q", gamma_q, T.f32, dev, (D,)),
+          _flat("gamma_k", gamma_k, T.f32, dev, (D,)), eps, c, s, rows, p, axes, struct.pack(f"@{axes}i", *pairs),
+          _code(dt))
     return q_out, k_out
-
-
-def _opt(t):
-    return None if t is None else t.data_ptr()
-
-
-def _workspace(n, device, stream):
-    """n bytes of device memory for one call on `stream` (None: the current one); freed in that stream's order."""
-    import torch
-
-    if not n:
-        return None
-    if stream is None:
-        return torch.empty(n, dtype=torch.uint8, device=device)
-    if isinstance(stream, int):
-        stream = torch.cuda.ExternalStream(stream, device=device)
-    with torch.cuda.stream(stream):
-        return torch.empty(n, dtype=torch.uint8, device=device)
-
-
-def _span(n) -> int:
-    """A window limit as the ABI takes it: 2^30 or more is none."""
-    return int(n) if n < (1 << 30) else -1
 
 
 class KVCache:
@@ -355,29 +362,31 @@ class KVCache:
     v_scale [seqs, kv_heads, slots, dim_head / 32, 2] (step and offset of each 32 channels).  The first `sinks`
     positions keep their slots, the other slots are a ring."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "sinks", "ring", "dtype", "device", "seqs", "kv_heads", "dim_head",
-                 "bits", "desc")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "sinks", "ring", "dtype", "device", "dev", "seqs", "kv_heads",
+                 "dim_head", "bits", "desc")
 
     def __init__(self, k, v, k_scale=None, v_scale=None, sinks=0):
-        import torch
-
-        self.bits = 4 if k.dtype == torch.uint8 else 0
-        _need(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype and k.device == v.device,
-              "k and v must be [seqs, kv_heads, slots, ...] of the same shape, type and device")
-        _need((k_scale is not None and v_scale is not None) == (self.bits == 4),
-              "k_scale and v_scale go with 4-bit (uint8) k and v")
-        _need(k.is_contiguous() and v.is_contiguous(), "k and v must be contiguous")
-        self.seqs, self.kv_heads, slots, width = k.shape
-        self.dim_head = 2 * width if self.bits else width
-        self.dtype, self.device = (k_scale.dtype if self.bits else k.dtype), k.device
-        if self.bits:
-            _need_flat(self.device, self.dtype, (self.seqs, self.kv_heads, slots, self.dim_head // 32, 2),
-                       k_scale=k_scale, v_scale=v_scale)
+        T = _torch()
+        dev = _device(k)
+        shape = k.shape
+        _need(len(shape) == 4, "k and v must be [seqs, kv_heads, slots, ...]")
+        seqs, kv_heads, slots, dim_head = shape
+        pk, pv = _flat("k", k, k.dtype, dev, shape), _flat("v", v, k.dtype, dev, shape)
+        _need(pk is not None and pv is not None, "k and v are needed")
+        bits, dtype, ps, qs = 0, k.dtype, 0, 0
+        if dtype is T.u8:
+            _need(k_scale is not None and v_scale is not None, "4-bit (uint8) k and v need k_scale and v_scale")
+            bits, dtype, dim_head = 4, k_scale.dtype, 2 * dim_head
+            sshape = (seqs, kv_heads, slots, dim_head // 32, 2)
+            ps, qs = _flat("k_scale", k_scale, dtype, dev, sshape), _flat("v_scale", v_scale, dtype, dev, sshape)
+        else:
+            _need(k_scale is None and v_scale is None, "k_scale and v_scale go with 4-bit (uint8) k and v")
+        sinks = int(sinks)
+        _need(0 <= sinks < slots, "a cache needs slots beyond its sinks")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.sinks, self.ring = int(sinks), slots - int(sinks)
-        _need(self.sinks >= 0 and self.ring >= 1, "a cache needs slots beyond its sinks")
-        self.desc = _CACHE.pack(k.data_ptr(), v.data_ptr(), _opt(k_scale) or 0, _opt(v_scale) or 0, self.seqs,
-                                self.kv_heads, self.dim_head, self.sinks, self.ring, _code(self.dtype), self.bits)
+        self.sinks, self.ring, self.dtype, self.device, self.dev = sinks, slots - sinks, dtype, k.device, dev
+        self.seqs, self.kv_heads, self.dim_head, self.bits = seqs, kv_heads, dim_head, bits
+        self.desc = _CACHE.pack(pk, pv, ps, qs, seqs, kv_heads, dim_head, sinks, slots - sinks, _code(dtype), bits)
 
     @classmethod
     def empty(cls, seqs, kv_heads, slots, dim_head, dtype, sinks=0, bits=0, device="cuda"):
@@ -395,46 +404,50 @@ class KVCache:
         return cls(k, v, ks, vs, sinks=sinks)
 
 
-def _code(dtype) -> int:
-    import torch
-
-    codes = {torch.float32: FP32, torch.float16: FP16, torch.bfloat16: BF16}
-    _need(dtype in codes, f"dtype must be float32, float16 or bfloat16, got {dtype}")
-    return codes[dtype]
-
-
 def op_cache_append(cache, k, v, pos, count=None, stream=None):
     """Writes tokens pos[s] + i, i < count[s] (None: all), of k, v [seqs, tokens, kv_heads, dim_head] into the cache;
     pos, count int32 [seqs]."""
-    import torch
-
-    _need_rows(cache.device, cache.dtype, k=k, v=v)
+    T, dev = _torch(), cache.dev
+    vk, vv = _rows("k", k, cache.dtype, dev), _rows("v", v, cache.dtype, dev)
     S, N, G, D = k.shape
     _need(v.shape == k.shape and S == cache.seqs and G == cache.kv_heads and D == cache.dim_head,
           "k and v must be [seqs, tokens, kv_heads, dim_head] of the cache")
     _need(pos is not None, "pos is needed")
-    _need_flat(cache.device, torch.int32, (S,), pos=pos, count=count)
-    with _on(cache.device):
-        _check(lib().mbr_op_cache_append(cache.desc, _view(k), _view(v), pos.data_ptr(), _opt(count), N,
-                                         _stream(stream)))
+    _call((_lib or lib()).mbr_op_cache_append, dev, stream, cache.desc, vk, vv, _flat("pos", pos, T.i32, dev, (S,)),
+          _flat("count", count, T.i32, dev, (S,)), N)
 
 
 def op_cache_read(cache, pos, tokens, count=None, k=None, v=None, stream=None):
     """Values of positions pos[s] + i, i < count[s] (None: tokens), the last of them being the newest of sequence s,
     as k, v [seqs, tokens, kv_heads, dim_head]; zeros where the cache holds nothing any more."""
-    import torch
-
-    shape = (cache.seqs, int(tokens), cache.kv_heads, cache.dim_head)
-    k = torch.empty(shape, dtype=cache.dtype, device=cache.device) if k is None else k
-    v = torch.empty(shape, dtype=cache.dtype, device=cache.device) if v is None else v
-    _need_rows(cache.device, cache.dtype, k=k, v=v)
-    _need(tuple(k.shape) == shape and tuple(v.shape) == shape, f"k and v must be {shape}")
+    T, dev, S = _torch(), cache.dev, cache.seqs
+    shape = (S, int(tokens), cache.kv_heads, cache.dim_head)
+    if k is None:
+        k = T.empty(shape, dtype=cache.dtype, device=cache.device)
+    if v is None:
+        v = T.empty(shape, dtype=cache.dtype, device=cache.device)
+    vk, vv = _rows("k", k, cache.dtype, dev), _rows("v", v, cache.dtype, dev)
+    _need(k.shape == shape and v.shape == shape, f"k and v must be {shape}")
     _need(pos is not None, "pos is needed")
-    _need_flat(cache.device, torch.int32, (cache.seqs,), pos=pos, count=count)
-    with _on(cache.device):
-        _check(lib().mbr_op_cache_read(cache.desc, pos.data_ptr(), _opt(count), shape[1], _view(k), _view(v),
-                                       _stream(stream)))
+    _call((_lib or lib()).mbr_op_cache_read, dev, stream, cache.desc, _flat("pos", pos, T.i32, dev, (S,)),
+          _flat("count", count, T.i32, dev, (S,)), shape[1], vk, vv)
     return k, v
+
+
+def _workspace(n, device, stream):
+    """n bytes of device memory for one call on `stream` (None: the current one); freed in that stream's order."""
+    torch = _T.torch
+    if stream is None:
+        return torch.empty(n, dtype=torch.uint8, device=device)
+    if isinstance(stream, int):
+        stream = torch.cuda.ExternalStream(stream, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def _span(n) -> int:
+    """A window limit as the ABI takes it: 2^30 or more is none."""
+    return int(n) if n < (1 << 30) else -1
 
 
 def op_window_attention(q, k, v, left=-1, right=-1, sinks=0, scale=0.0, q_len=None, kv_len=None, gates=None, out=None,
@@ -443,47 +456,48 @@ def op_window_attention(q, k, v, left=-1, right=-1, sinks=0, scale=0.0, q_len=No
     limit) and the first `sinks`, times gates [seqs, q_tokens, q_heads] if given.  q [seqs, q_tokens, q_heads,
     dim_head], k, v [seqs, kv_tokens, kv_heads, dim_head] (views allowed); q_len, kv_len int32 [seqs]: the queries are
     the last q_len[s] of the kv_len[s] tokens of sequence s.  -> [seqs, q_tokens, q_heads, dim_head]."""
-    import torch
-
+    T = _torch()
+    dev, dt = _device(q), q.dtype
+    vq, vk, vv = _rows("q", q, dt, dev), _rows("k", k, dt, dev), _rows("v", v, dt, dev)
     S, N, H, D = q.shape
-    dev, dt = q.device, q.dtype
-    out = torch.empty((S, N, H, D), dtype=dt, device=dev) if out is None else out
-    _need_rows(dev, dt, q=q, k=k, v=v, out=out)
     M, G = k.shape[1], k.shape[2]
     _need(k.shape == v.shape and k.shape[0] == S and k.shape[3] == D, "k and v must be [seqs, kv_tokens, kv_heads, D]")
+    if out is None:
+        out = T.empty((S, N, H, D), dtype=dt, device=q.device)
     _need(out.shape == q.shape, "out must have the shape of q")
-    _need_flat(dev, torch.int32, (S,), q_len=q_len, kv_len=kv_len)
-    _need_flat(dev, torch.float32, (S, N, H), gates=gates)
-    left, right, sinks, n = _span(left), _span(right), min(int(sinks), 1 << 30), ctypes.c_int64()
-    _check(lib().mbr_op_window_attention_workspace(S, N, M, H, G, D, left, right, sinks, _dt(q), ctypes.byref(n)))
-    with _on(dev):
-        work = _workspace(n.value, dev, stream)
-        _check(lib().mbr_op_window_attention(
-            _view(q), _view(k), _view(v), _view(out), S, N, M, H, G, D, _opt(q_len), _opt(kv_len), left, right, sinks,
-            scale, _opt(gates), _dt(q), _opt(work), n.value, _stream(stream)))
+    left, right, sinks, code = _span(left), _span(right), min(int(sinks), 1 << 30), _code(dt)
+    L, work, n = _lib or lib(), None, 0
+    if N <= 64:  # the form for few queries may need memory of its own
+        size = ctypes.c_int64()
+        _check(L.mbr_op_window_attention_workspace(S, N, M, H, G, D, left, right, sinks, code, ctypes.byref(size)))
+        n = size.value
+        work = _workspace(n, q.device, stream) if n else None
+    _call(L.mbr_op_window_attention, dev, stream, vq, vk, vv, _rows("out", out, dt, dev), S, N, M, H, G, D,
+          _flat("q_len", q_len, T.i32, dev, (S,)), _flat("kv_len", kv_len, T.i32, dev, (S,)), left, right, sinks, scale,
+          _flat("gates", gates, T.f32, dev, (S, N, H)), code, work.data_ptr() if n else None, n)
     return out
 
 
 def op_cache_attention(q, cache, length, left=-1, right=0, scale=0.0, gates=None, out=None, stream=None):
     """The attention of op_window_attention for the newest tokens over a cache that holds them: q [seqs, tokens,
     q_heads, dim_head], length int32 [seqs] tokens appended so far (these included); the cache's sinks stay visible."""
-    import torch
-
+    T, dev, dt = _torch(), cache.dev, cache.dtype
+    vq = _rows("q", q, dt, dev)
     S, N, H, D = q.shape
-    dev = cache.device
-    out = torch.empty((S, N, H, D), dtype=q.dtype, device=dev) if out is None else out
-    _need_rows(dev, cache.dtype, q=q, out=out)
     _need(S == cache.seqs and D == cache.dim_head, "q must be [seqs, tokens, q_heads, dim_head] of the cache")
+    if out is None:
+        out = T.empty((S, N, H, D), dtype=dt, device=cache.device)
     _need(out.shape == q.shape, "out must have the shape of q")
     _need(length is not None, "length is needed")
-    _need_flat(dev, torch.int32, (S,), length=length)
-    _need_flat(dev, torch.float32, (S, N, H), gates=gates)
-    left, right, n = _span(left), _span(right), ctypes.c_int64()
-    _check(lib().mbr_op_cache_attention_workspace(cache.desc, N, H, left, right, ctypes.byref(n)))
-    with _on(dev):
-        work = _workspace(n.value, dev, stream)
-        _check(lib().mbr_op_cache_attention(_view(q), cache.desc, _view(out), length.data_ptr(), N, H, left, right, scale,
-                                            _opt(gates), _opt(work), n.value, _stream(stream)))
+    left, right, size = _span(left), _span(right), ctypes.c_int64()
+    L, work = _lib or lib(), None
+    _check(L.mbr_op_cache_attention_workspace(cache.desc, N, H, left, right, ctypes.byref(size)))
+    n = size.value
+    if n:
+        work = _workspace(n, cache.device, stream)
+    _call(L.mbr_op_cache_attention, dev, stream, vq, cache.desc, _rows("out", out, dt, dev),
+          _flat("length", length, T.i32, dev, (S,)), N, H, left, right, scale,
+          _flat("gates", gates, T.f32, dev, (S, N, H)), work.data_ptr() if n else None, n)
     return out
 
 

@@ -79,7 +79,7 @@ def test_entry_points_refuse_without_a_gpu():
                append(cache(bits=4, D=40)), append(cache(ring=0)), append(cache(sinks=-1)), append(cache(D=4)),
                append(cache(k=4104)), append(cache(), tokens=-1), append(cache(), pos=None),
                L.mbr_op_cache_attention(view, cache(), view, None, 1, 1, -1, 0, 0.0, None, None, 0, None),
-               L.mbr_op_cache_attention(view, cache(), view, one, 1, 1, -1, 0, 0.0, None, None, 0, None),
+               L.mbr_op_cache_attention(view, cache(ring=100000), view, one, 1, 1, -1, 0, 0.0, None, None, 0, None),
                L.mbr_op_cache_attention(view, None, view, one, 1, 1, -1, 0, 0.0, None, None, 0, None)]
     assert refused == [1] * len(refused)
     assert L.mbr_last_error()
