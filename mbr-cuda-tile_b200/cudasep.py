@@ -10,7 +10,6 @@ from __future__ import annotations
 
 import ctypes
 import os
-import struct
 
 import numpy as np
 
@@ -242,85 +241,57 @@ def op_attention(q, k, v, scale=0.0, gates=None, out=None, stream=None):
 
 
 # ---- streaming time-axis attention ----
-# A frame's kernels take two or three microseconds, so what these wrappers do per
-# call is kept short: each tensor is looked at once, its view packed on the spot.
-_VIEW = struct.Struct("@Pqqq")  # mbr_view
-_CACHE = struct.Struct("@PPPPqiiiiii")  # mbr_kv_cache
-_T = None  # torch and what is used of it per call, see _torch()
+_CALLS = None  # the extension that makes these calls, see _calls()
 
 
-class _Torch:
-    """torch's names that the streaming operators use per call."""
+def _calls():
+    """The streaming operators' calls (binding/stream_calls.c), bound to the library and torch on first use.  A frame's
+    kernels take two or three microseconds, so the tensors are looked at and the arguments converted in C."""
+    global _CALLS
+    if _CALLS is None:
+        import importlib.util
 
-    def __init__(self):
         import torch
 
-        self.torch = torch
-        self.empty = torch.empty
-        self.codes = {torch.float32: FP32, torch.float16: FP16, torch.bfloat16: BF16}
-        self.f32, self.i32, self.u8 = torch.float32, torch.int32, torch.uint8
-        self.current_device = torch.cuda.current_device
-        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # the stream's handle without a Stream object
-        self.raw_stream = raw or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+        path = os.path.join(HERE, "_stream_calls.so")
+        if not os.path.exists(path):
+            raise ImportError(f"{path} is missing: build it with `make -C {HERE}` (or __graft_entry__.build())")
+        spec = importlib.util.spec_from_file_location("_stream_calls", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        names = ("mbr_op_qk_norm_rope", "mbr_op_cache_append", "mbr_op_cache_read", "mbr_op_window_attention",
+                 "mbr_op_window_attention_workspace", "mbr_op_cache_attention", "mbr_op_cache_attention_workspace")
+        L = lib()
+        # torch's functions without the Python layers above them, where this version has them
+        stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                         lambda device: torch.cuda.current_stream(device).cuda_stream)
+        device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+        module.bind(
+            tuple(ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in names),
+            (torch.float32, torch.int32, torch.uint8, {torch.float32: FP32, torch.float16: FP16, torch.bfloat16: BF16},
+             torch.empty_like, {"memory_format": torch.contiguous_format}, stream, device, _check, _elsewhere, _workspace))
+        _CALLS = module
+    return _CALLS
 
 
-def _torch() -> _Torch:
-    global _T
-    if _T is None:
-        _T = _Torch()
-    return _T
+def _elsewhere(dev, name, args):
+    """A call of the extension with another device made current."""
+    import torch
+
+    with torch.cuda.device(dev):
+        return getattr(_CALLS, name)(*args)
 
 
-def _need(cond, msg):
-    if not cond:
-        raise ValueError(msg)
+def _workspace(n, device, stream):
+    """n bytes of device memory for one call on `stream` (None: the current one); freed in that stream's order."""
+    import torch
 
-
-def _rows(name, t, dtype, dev) -> bytes:
-    """mbr_view of a [seqs, tokens, heads, dim_head] tensor of this type on this device, last axis contiguous."""
-    st = t.stride()
-    if len(st) != 4 or t.dtype is not dtype or t.get_device() != dev or (st[3] != 1 and t.shape[3] > 1):
-        raise ValueError(f"{name} must be [seqs, tokens, heads, dim_head] of {dtype} on cuda:{dev} with a contiguous "
-                         f"last axis, got {tuple(t.shape)} of {t.dtype} on {t.device}")
-    return _VIEW.pack(t.data_ptr(), st[0], st[1], st[2])
-
-
-def _flat(name, t, dtype, dev, shape):
-    """Address of a contiguous tensor of this type and shape on this device; None if there is none."""
-    if t is None:
-        return None
-    if t.dtype is not dtype or t.get_device() != dev or t.shape != shape or not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous {dtype} of shape {shape} on cuda:{dev}, "
-                         f"got {tuple(t.shape)} of {t.dtype} on {t.device}")
-    return t.data_ptr()
-
-
-def _device(t) -> int:
-    dev = t.get_device()
-    _need(dev >= 0, f"tensors must be on a CUDA device, got {t.device}")
-    return dev
-
-
-def _call(fn, dev, stream, *args):
-    """fn(*args, stream) with `dev` current; stream None is torch's current one there."""
-    T = _T
     if stream is None:
-        stream = T.raw_stream(dev)
-    elif not isinstance(stream, int):
-        stream = stream.cuda_stream
-    if T.current_device() == dev:
-        rc = fn(*args, stream)
-    else:
-        with T.torch.cuda.device(dev):
-            rc = fn(*args, stream)
-    if rc:
-        _check(rc)
-
-
-def _code(dtype) -> int:
-    code = _torch().codes.get(dtype)
-    _need(code is not None, f"dtype must be float32, float16 or bfloat16, got {dtype}")
-    return code
+        return torch.empty(n, dtype=torch.uint8, device=device)
+    if isinstance(stream, int):
+        stream = torch.cuda.ExternalStream(stream, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(n, dtype=torch.uint8, device=device)
 
 
 def op_qk_norm_rope(q, k, gamma_q=None, gamma_k=None, cos=None, sin=None, pos=None, pairs=(), eps=1e-6, q_out=None,
@@ -329,30 +300,7 @@ def op_qk_norm_rope(q, k, gamma_q=None, gamma_k=None, cos=None, sin=None, pos=No
     (x / sqrt(mean x^2 + eps) * gamma) and rotated: pairs[a] pairs (2i, 2i+1) turn by row pos[s, t, a] of the tables
     cos, sin [rows, dim_head / 2].  pos int32 [seqs, tokens, len(pairs)].  q, k may be strided views (last axis
     contiguous); q_out / k_out may be q / k themselves."""
-    T = _torch()
-    dev, dt = _device(q), q.dtype
-    vq, vk = _rows("q", q, dt, dev), _rows("k", k, dt, dev)
-    S, N, H, D = q.shape
-    ks = k.shape
-    G = ks[2]
-    _need(ks == (S, N, G, D), "q and k must have the same seqs, tokens, dim_head")
-    if q_out is None:
-        q_out = T.empty((S, N, H, D), dtype=dt, device=q.device)
-    if k_out is None:
-        k_out = T.empty((S, N, G, D), dtype=dt, device=q.device)
-    _need(q_out.shape == q.shape and k_out.shape == ks, "outputs must have the shapes of q and k")
-    axes = len(pairs)
-    rows, c, s, p = 0, None, None, None
-    if axes:
-        _need(cos is not None and sin is not None and pos is not None, "cos, sin and pos are needed with pairs")
-        rows = cos.shape[0]
-        c, s = _flat("cos", cos, T.f32, dev, (rows, D // 2)), _flat("sin", sin, T.f32, dev, (rows, D // 2))
-        p = _flat("pos", pos, T.i32, dev, (S, N, axes))
-    _call((_lib or lib()).mbr_op_qk_norm_rope, dev, stream, vq, vk, _rows("q_out", q_out, dt, dev),
-          _rows("k_out", k_out, dt, dev), S, N, H, G, D, _flat("gamma_q", gamma_q, T.f32, dev, (D,)),
-          _flat("gamma_k", gamma_k, T.f32, dev, (D,)), eps, c, s, rows, p, axes, struct.pack(f"@{axes}i", *pairs),
-          _code(dt))
-    return q_out, k_out
+    return (_CALLS or _calls()).qk_norm_rope(q, k, gamma_q, gamma_k, cos, sin, pos, pairs, eps, q_out, k_out, stream)
 
 
 class KVCache:
@@ -362,31 +310,17 @@ class KVCache:
     v_scale [seqs, kv_heads, slots, dim_head / 32, 2] (step and offset of each 32 channels).  The first `sinks`
     positions keep their slots, the other slots are a ring."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "sinks", "ring", "dtype", "device", "dev", "seqs", "kv_heads",
-                 "dim_head", "bits", "desc")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "sinks", "ring", "dtype", "dev", "seqs", "kv_heads", "dim_head", "bits",
+                 "desc")
 
     def __init__(self, k, v, k_scale=None, v_scale=None, sinks=0):
-        T = _torch()
-        dev = _device(k)
-        shape = k.shape
-        _need(len(shape) == 4, "k and v must be [seqs, kv_heads, slots, ...]")
-        seqs, kv_heads, slots, dim_head = shape
-        pk, pv = _flat("k", k, k.dtype, dev, shape), _flat("v", v, k.dtype, dev, shape)
-        _need(pk is not None and pv is not None, "k and v are needed")
-        bits, dtype, ps, qs = 0, k.dtype, 0, 0
-        if dtype is T.u8:
-            _need(k_scale is not None and v_scale is not None, "4-bit (uint8) k and v need k_scale and v_scale")
-            bits, dtype, dim_head = 4, k_scale.dtype, 2 * dim_head
-            sshape = (seqs, kv_heads, slots, dim_head // 32, 2)
-            ps, qs = _flat("k_scale", k_scale, dtype, dev, sshape), _flat("v_scale", v_scale, dtype, dev, sshape)
-        else:
-            _need(k_scale is None and v_scale is None, "k_scale and v_scale go with 4-bit (uint8) k and v")
-        sinks = int(sinks)
-        _need(0 <= sinks < slots, "a cache needs slots beyond its sinks")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.sinks, self.ring, self.dtype, self.device, self.dev = sinks, slots - sinks, dtype, k.device, dev
-        self.seqs, self.kv_heads, self.dim_head, self.bits = seqs, kv_heads, dim_head, bits
-        self.desc = _CACHE.pack(pk, pv, ps, qs, seqs, kv_heads, dim_head, sinks, slots - sinks, _code(dtype), bits)
+        (self.desc, self.dtype, self.dev, self.seqs, self.kv_heads, self.dim_head, self.ring,
+         self.bits) = (_CALLS or _calls()).cache_fields(k, v, k_scale, v_scale, sinks)
+        self.k, self.v, self.k_scale, self.v_scale, self.sinks = k, v, k_scale, v_scale, sinks
+
+    def new(self, shape):
+        """An uninitialised tensor of the cache's type on its device."""
+        return (self.k_scale if self.bits else self.k).new_empty(shape)
 
     @classmethod
     def empty(cls, seqs, kv_heads, slots, dim_head, dtype, sinks=0, bits=0, device="cuda"):
@@ -396,7 +330,8 @@ class KVCache:
         if not bits:
             k, v = (torch.zeros((seqs, kv_heads, slots, dim_head), dtype=dtype, device=device) for _ in range(2))
             return cls(k, v, sinks=sinks)
-        _need(bits == 4, "bits must be 0 or 4")
+        if bits != 4:
+            raise ValueError("bits must be 0 or 4")
         k, v = (torch.zeros((seqs, kv_heads, slots, dim_head // 2), dtype=torch.uint8, device=device)
                 for _ in range(2))
         ks, vs = (torch.zeros((seqs, kv_heads, slots, dim_head // 32, 2), dtype=dtype, device=device)
@@ -407,47 +342,13 @@ class KVCache:
 def op_cache_append(cache, k, v, pos, count=None, stream=None):
     """Writes tokens pos[s] + i, i < count[s] (None: all), of k, v [seqs, tokens, kv_heads, dim_head] into the cache;
     pos, count int32 [seqs]."""
-    T, dev = _torch(), cache.dev
-    vk, vv = _rows("k", k, cache.dtype, dev), _rows("v", v, cache.dtype, dev)
-    S, N, G, D = k.shape
-    _need(v.shape == k.shape and S == cache.seqs and G == cache.kv_heads and D == cache.dim_head,
-          "k and v must be [seqs, tokens, kv_heads, dim_head] of the cache")
-    _need(pos is not None, "pos is needed")
-    _call((_lib or lib()).mbr_op_cache_append, dev, stream, cache.desc, vk, vv, _flat("pos", pos, T.i32, dev, (S,)),
-          _flat("count", count, T.i32, dev, (S,)), N)
+    (_CALLS or _calls()).cache_append(cache, k, v, pos, count, stream)
 
 
 def op_cache_read(cache, pos, tokens, count=None, k=None, v=None, stream=None):
     """Values of positions pos[s] + i, i < count[s] (None: tokens), the last of them being the newest of sequence s,
     as k, v [seqs, tokens, kv_heads, dim_head]; zeros where the cache holds nothing any more."""
-    T, dev, S = _torch(), cache.dev, cache.seqs
-    shape = (S, int(tokens), cache.kv_heads, cache.dim_head)
-    if k is None:
-        k = T.empty(shape, dtype=cache.dtype, device=cache.device)
-    if v is None:
-        v = T.empty(shape, dtype=cache.dtype, device=cache.device)
-    vk, vv = _rows("k", k, cache.dtype, dev), _rows("v", v, cache.dtype, dev)
-    _need(k.shape == shape and v.shape == shape, f"k and v must be {shape}")
-    _need(pos is not None, "pos is needed")
-    _call((_lib or lib()).mbr_op_cache_read, dev, stream, cache.desc, _flat("pos", pos, T.i32, dev, (S,)),
-          _flat("count", count, T.i32, dev, (S,)), shape[1], vk, vv)
-    return k, v
-
-
-def _workspace(n, device, stream):
-    """n bytes of device memory for one call on `stream` (None: the current one); freed in that stream's order."""
-    torch = _T.torch
-    if stream is None:
-        return torch.empty(n, dtype=torch.uint8, device=device)
-    if isinstance(stream, int):
-        stream = torch.cuda.ExternalStream(stream, device=device)
-    with torch.cuda.stream(stream):
-        return torch.empty(n, dtype=torch.uint8, device=device)
-
-
-def _span(n) -> int:
-    """A window limit as the ABI takes it: 2^30 or more is none."""
-    return int(n) if n < (1 << 30) else -1
+    return (_CALLS or _calls()).cache_read(cache, pos, tokens, count, k, v, stream)
 
 
 def op_window_attention(q, k, v, left=-1, right=-1, sinks=0, scale=0.0, q_len=None, kv_len=None, gates=None, out=None,
@@ -456,49 +357,13 @@ def op_window_attention(q, k, v, left=-1, right=-1, sinks=0, scale=0.0, q_len=No
     limit) and the first `sinks`, times gates [seqs, q_tokens, q_heads] if given.  q [seqs, q_tokens, q_heads,
     dim_head], k, v [seqs, kv_tokens, kv_heads, dim_head] (views allowed); q_len, kv_len int32 [seqs]: the queries are
     the last q_len[s] of the kv_len[s] tokens of sequence s.  -> [seqs, q_tokens, q_heads, dim_head]."""
-    T = _torch()
-    dev, dt = _device(q), q.dtype
-    vq, vk, vv = _rows("q", q, dt, dev), _rows("k", k, dt, dev), _rows("v", v, dt, dev)
-    S, N, H, D = q.shape
-    M, G = k.shape[1], k.shape[2]
-    _need(k.shape == v.shape and k.shape[0] == S and k.shape[3] == D, "k and v must be [seqs, kv_tokens, kv_heads, D]")
-    if out is None:
-        out = T.empty((S, N, H, D), dtype=dt, device=q.device)
-    _need(out.shape == q.shape, "out must have the shape of q")
-    left, right, sinks, code = _span(left), _span(right), min(int(sinks), 1 << 30), _code(dt)
-    L, work, n = _lib or lib(), None, 0
-    if N <= 64:  # the form for few queries may need memory of its own
-        size = ctypes.c_int64()
-        _check(L.mbr_op_window_attention_workspace(S, N, M, H, G, D, left, right, sinks, code, ctypes.byref(size)))
-        n = size.value
-        work = _workspace(n, q.device, stream) if n else None
-    _call(L.mbr_op_window_attention, dev, stream, vq, vk, vv, _rows("out", out, dt, dev), S, N, M, H, G, D,
-          _flat("q_len", q_len, T.i32, dev, (S,)), _flat("kv_len", kv_len, T.i32, dev, (S,)), left, right, sinks, scale,
-          _flat("gates", gates, T.f32, dev, (S, N, H)), code, work.data_ptr() if n else None, n)
-    return out
+    return (_CALLS or _calls()).window_attention(q, k, v, left, right, sinks, scale, q_len, kv_len, gates, out, stream)
 
 
 def op_cache_attention(q, cache, length, left=-1, right=0, scale=0.0, gates=None, out=None, stream=None):
     """The attention of op_window_attention for the newest tokens over a cache that holds them: q [seqs, tokens,
     q_heads, dim_head], length int32 [seqs] tokens appended so far (these included); the cache's sinks stay visible."""
-    T, dev, dt = _torch(), cache.dev, cache.dtype
-    vq = _rows("q", q, dt, dev)
-    S, N, H, D = q.shape
-    _need(S == cache.seqs and D == cache.dim_head, "q must be [seqs, tokens, q_heads, dim_head] of the cache")
-    if out is None:
-        out = T.empty((S, N, H, D), dtype=dt, device=cache.device)
-    _need(out.shape == q.shape, "out must have the shape of q")
-    _need(length is not None, "length is needed")
-    left, right, size = _span(left), _span(right), ctypes.c_int64()
-    L, work = _lib or lib(), None
-    _check(L.mbr_op_cache_attention_workspace(cache.desc, N, H, left, right, ctypes.byref(size)))
-    n = size.value
-    if n:
-        work = _workspace(n, cache.device, stream)
-    _call(L.mbr_op_cache_attention, dev, stream, vq, cache.desc, _rows("out", out, dt, dev),
-          _flat("length", length, T.i32, dev, (S,)), N, H, left, right, scale,
-          _flat("gates", gates, T.f32, dev, (S, N, H)), work.data_ptr() if n else None, n)
-    return out
+    return (_CALLS or _calls()).cache_attention(q, cache, length, left, right, scale, gates, out, stream)
 
 
 def op_stft(sig, hop=441, stream=None):

@@ -1,6 +1,6 @@
 """CPU checks of the references that the streaming-attention tests use, and of the C entry points' argument checks."""
-import ctypes
 import math
+import struct
 
 import numpy as np
 import pytest
@@ -56,7 +56,7 @@ def test_entry_points_refuse_without_a_gpu():
 
     L = cudasep.lib()
     one = np.zeros(64, np.float32).ctypes.data
-    view = cudasep._VIEW.pack(one, 64, 64, 64)
+    view = struct.pack("@Pqqq", one, 64, 64, 64)
 
     def norm(D=64, axes=0, pairs=None, eps=1e-6, dtype=1, seqs=1):
         return L.mbr_op_qk_norm_rope(view, view, view, view, seqs, 1, 1, 1, D, None, None, eps, None, None, 0, None, axes,
@@ -67,7 +67,7 @@ def test_entry_points_refuse_without_a_gpu():
                                          dtype, None, 0, None)
 
     def cache(dtype=1, bits=0, D=64, ring=4, sinks=0, k=4096):
-        return cudasep._CACHE.pack(k, k, k if bits else 0, k if bits else 0, 1, 1, D, sinks, ring, dtype, bits)
+        return struct.pack("@PPPPqiiiiii", k, k, k if bits else 0, k if bits else 0, 1, 1, D, sinks, ring, dtype, bits)
 
     def append(c, tokens=1, pos=one):
         return L.mbr_op_cache_append(c, view, view, pos, None, tokens, None)
@@ -87,15 +87,14 @@ def test_entry_points_refuse_without_a_gpu():
     assert window(N=0) == 0 and norm(seqs=0) == 0 and append(cache(), tokens=0) == 0
 
 
-def test_views_and_caches_have_the_abi_size():
+def test_the_extension_refuses_cpu_tensors():
+    """The Python calls check their tensors before anything else happens."""
     import cudasep
 
-    class View(ctypes.Structure):
-        _fields_ = [("data", ctypes.c_void_p), ("seq", ctypes.c_int64), ("token", ctypes.c_int64),
-                    ("head", ctypes.c_int64)]
-
-    class Cache(ctypes.Structure):
-        _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + [("seqs", ctypes.c_int64)] + [
-            (n, ctypes.c_int) for n in ("kv_heads", "dim_head", "sinks", "ring", "dtype", "bits")]
-
-    assert cudasep._VIEW.size == ctypes.sizeof(View) and cudasep._CACHE.size == ctypes.sizeof(Cache)
+    x = torch.zeros(1, 2, 3, 64)
+    for call in (lambda: cudasep.op_qk_norm_rope(x, x), lambda: cudasep.op_window_attention(x, x, x),
+                 lambda: cudasep.KVCache(x, x), lambda: cudasep.KVCache(None, None)):
+        with pytest.raises((ValueError, AttributeError)):
+            call()
+    with pytest.raises(ValueError):
+        cudasep.KVCache.empty(1, 1, 8, 64, torch.float16, bits=3, device="cpu")
