@@ -388,39 +388,43 @@ __global__ void __launch_bounds__(160, TileCfg<DH>::CTAS)
                 };
                 float rs = 0.f;
                 bool low = see != 0 && m == -INFINITY;
-                if (!__any_sync(0xffffffffu, low)) {
-                    rs = weights(m == -INFINITY ? 0.f : m);
-                    low = sees && !(rs <= kRescaleSum);  // inf and NaN too
-                }
-                if (__any_sync(0xffffffffu, low)) {
-                    float top = -INFINITY;
-#pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        if (!(need >> q & 1)) continue;
-                        uint32_t sv[32];
-                        tmem_ld32(tS + 32 * q, sv);
-                        tmem_ld_wait(sv);
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (half[q] >> i & 1) top = fmaxf(top, __uint_as_float(sv[i]) * c);
-                    }
-                    const float now = low ? fmaxf(m, top) : m;
-                    const float f = now == m ? 1.f : ex2_approx(m - now);
-                    m = now;
-                    l *= f;
-                    if (j > 0) {  // O holds the blocks before: every product issued before S(g) is done
 #pragma unroll 1
-                        for (int q = 0; q < 4 * DH; ++q) {
-                            uint32_t ov[16];
-                            tmem_ld16(tO + 16 * q, ov);
+                for (int pass = 0; pass < 3; ++pass) {
+                    if (__any_sync(0xffffffffu, low)) {
+                        float top = -INFINITY;
+#pragma unroll 1
+                        for (int q = 0; q < 4; ++q) {
+                            if (!(need >> (q >> 1) & 1)) continue;
+                            uint32_t sv[16];
+                            tmem_ld16(tS + 16 * q, sv);
                             tmem_ld_wait();
+                            const uint32_t bits = half[q >> 1] >> (16 * (q & 1));
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * f);
-                            tmem_st16(tO + 16 * q, ov);
+                            for (int i = 0; i < 16; ++i)
+                                if (bits >> i & 1) top = fmaxf(top, __uint_as_float(sv[i]) * c);
                         }
-                        tmem_st_wait();
+                        const float now = low ? fmaxf(m, top) : m;
+                        const float f = now == m ? 1.f : ex2_approx(m - now);
+                        m = now;
+                        const bool scaled = j > 0 && f != 1.f && l != 0.f;
+                        l *= f;
+                        if (__any_sync(0xffffffffu, scaled)) {
+#pragma unroll 1
+                            for (int q = 0; q < 4 * DH; ++q) {
+                                uint32_t ov[16];
+                                tmem_ld16(tO + 16 * q, ov);
+                                tmem_ld_wait();
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * f);
+                                tmem_st16(tO + 16 * q, ov);
+                            }
+                            tmem_st_wait();
+                        }
+                    } else if (pass > 0) {
+                        break;
                     }
                     rs = weights(m == -INFINITY ? 0.f : m);
+                    low = pass < 1 && sees && !(rs <= kRescaleSum);
                 }
                 l += rs;
                 tmem_st32(tS, pk);  // over the first half of S, which this warp has read
