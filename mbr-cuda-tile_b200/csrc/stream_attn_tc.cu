@@ -335,20 +335,30 @@ __global__ void __launch_bounds__(160, TileCfg<DH>::CTAS)
             const bool sees = w.hi > w.lo || w.first > 0;
             const int h = x.h0 + rh;
             const float gate = valid && a.gates ? __ldg(a.gates + ((int64_t)x.s * a.Nq + token) * a.Hq + h) : 1.f;
+            // keys that every row of this warp (that sees any) sees
+            const int all_lo = __reduce_max_sync(0xffffffffu, sees ? w.lo : 0);
+            const int all_hi = __reduce_min_sync(0xffffffffu, sees ? w.hi : INT32_MAX);
             float m = -INFINITY, l = 0.f;
             for (int j = 0; j < x.nkv; ++j, ++g) {
                 const int key = block_key(x, j);
-                // columns this row sees: a first-token block holds only those before the window
-                uint64_t see = j < x.nsb ? bits_between(0, min(w.first, x.ns) - key)
-                                         : bits_between(w.lo - key, w.hi - key) | bits_between(0, w.first - key);
-                if (!sees) see = 0;
-                const uint32_t half[2] = {(uint32_t)see, (uint32_t)(see >> 32)};
-                uint32_t need = 0, whole = 0;  // chunks that some row sees; that every row (that is one) sees whole
+                // columns this row sees (a first-token block holds only those before the window); chunks that some
+                // row sees; chunks that every row (that sees any key) sees whole
+                uint64_t see = sees ? ~0ull : 0ull;
+                uint32_t need = 3, whole = 3;
+                if (j < x.nsb || key < all_lo || key + KB > all_hi) {
+                    see = j < x.nsb ? bits_between(0, min(w.first, x.ns) - key)
+                                    : bits_between(w.lo - key, w.hi - key) | bits_between(0, w.first - key);
+                    if (!sees) see = 0;
+                    need = whole = 0;
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    if (__any_sync(0xffffffffu, half[q] != 0u)) need |= 1u << q;
-                    if ((need >> q & 1) && __all_sync(0xffffffffu, half[q] == 0xffffffffu || !sees)) whole |= 1u << q;
+                    for (int q = 0; q < 2; ++q) {
+                        const uint32_t part = (uint32_t)(see >> (32 * q));
+                        if (__any_sync(0xffffffffu, part != 0u)) need |= 1u << q;
+                        if (__all_sync(0xffffffffu, part == 0xffffffffu || !sees)) whole |= 1u << q;
+                    }
+                    whole &= need;
                 }
+                const uint32_t half[2] = {(uint32_t)see, (uint32_t)(see >> 32)};
                 ok = __all_sync(0xffffffffu, mbar_wait(bar_s, g & 1, p.err));
                 if (!ok) break;
                 tc_fence_after();
@@ -356,20 +366,20 @@ __global__ void __launch_bounds__(160, TileCfg<DH>::CTAS)
                 // weights with offset mo as 16-bit pairs; returns this row's sum.  A chunk's scores are loaded
                 // when it comes to them: two at once would not leave registers for three CTAs.
                 auto weights = [&](float mo) {
-                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
                     uint32_t sv[32];
                     auto chunk = [&](int q, auto all) {
 #pragma unroll
                         for (int i = 0; i < 32; i += 2) {
-                            float e0 = ex2_approx(fmaf(__uint_as_float(sv[i]), c, -mo));
-                            float e1 = ex2_approx(fmaf(__uint_as_float(sv[i + 1]), c, -mo));
+                            const float2 z = __ffma2_rn(make_float2(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1])),
+                                                        make_float2(c, c), make_float2(-mo, -mo));
+                            float2 e = make_float2(ex2_approx(z.x), ex2_approx(z.y));
                             if constexpr (!decltype(all)::value) {
-                                e0 = half[q] >> i & 1 ? e0 : 0.f;
-                                e1 = half[q] >> (i + 1) & 1 ? e1 : 0.f;
+                                e.x = half[q] >> i & 1 ? e.x : 0.f;
+                                e.y = half[q] >> (i + 1) & 1 ? e.y : 0.f;
                             }
-                            sum[i & 2] += e0;
-                            sum[(i & 2) + 1] += e1;
-                            pk[16 * q + i / 2] = pack2(e0, e1, (T*)nullptr);
+                            sum[i / 2 & 1] = __fadd2_rn(sum[i / 2 & 1], e);
+                            pk[16 * q + i / 2] = pack2(e.x, e.y, (T*)nullptr);
                         }
                     };
 #pragma unroll
@@ -384,7 +394,7 @@ __global__ void __launch_bounds__(160, TileCfg<DH>::CTAS)
                             for (int i = 0; i < 16; ++i) pk[16 * q + i] = 0u;
                         }
                     }
-                    return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    return (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 };
                 float rs = 0.f;
                 bool low = see != 0 && m == -INFINITY;
@@ -529,7 +539,11 @@ void launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, co
         MBR_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::TOTAL));
         MBR_CUDA(cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev));
     }
-    const unsigned grid = std::min<unsigned>(p.ntiles, (unsigned)(sms[dev] * Cfg::CTAS));
+    // Persistent CTAs take tiles in turn and load the next one's Q behind the last product (the 8 s chunk: 99 us against
+    // 119 with a CTA a tile).  With lengths given, what a tile holds is not known here: a CTA a tile, so that the
+    // hardware evens it out (ragged pieces: 58 us against 63).
+    const unsigned grid =
+        p.a.q_len || p.a.kv_len ? p.ntiles : std::min<unsigned>(p.ntiles, (unsigned)(sms[dev] * Cfg::CTAS));
     kern<<<grid, 160, Cfg::TOTAL, st>>>(q, k, v, p);
     MBR_CUDA(cudaGetLastError());
 }
