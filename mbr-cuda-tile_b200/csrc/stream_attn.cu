@@ -102,8 +102,8 @@ AttnArgs window_args(const mbr_view& q, const mbr_view& k, const mbr_view& v, co
 // The form for few queries: rows that fit its tiles a few times over.
 bool few_rows(const AttnArgs& a) { return (int64_t)a.Nq * a.G <= 64; }
 
-StepPlan plan_of(const AttnArgs& a, int64_t held) {
-    return step_plan(a.seqs, a.Nq, a.Hq, a.Hkv, a.D, most_keys(a, held));
+StepPlan plan_of(const AttnArgs& a, bool q4, int64_t held) {
+    return step_plan(a.seqs, a.Nq, a.Hq, a.Hkv, a.D, q4, most_keys(a, held));
 }
 
 }  // namespace
@@ -114,7 +114,7 @@ int64_t window_attention_workspace(int64_t seqs, int64_t Nq, int64_t Nk, int Hq,
     const AttnArgs a =
         window_args(none, none, none, none, seqs, Nq, Nk, Hq, Hkv, D, left, right, sinks, 0.f, nullptr, dtype);
     if (seqs == 0 || Nq == 0 || Hq == 0 || dtype == DT_F32 || !few_rows(a)) return 0;
-    return plan_of(a, Nk).bytes;
+    return plan_of(a, false, Nk).bytes;
 }
 
 void window_attention(const mbr_view& q, const mbr_view& k, const mbr_view& v, const mbr_view& out, int64_t seqs,
@@ -126,7 +126,7 @@ void window_attention(const mbr_view& q, const mbr_view& k, const mbr_view& v, c
     MBR_CHECK(q.data && out.data && (Nk == 0 || (k.data && v.data)), "window_attention: null buffer");
     a.q_len = q_len, a.kv_len = kv_len;
     if (few_rows(a) && step_supported(a, dtype, false)) {
-        const StepPlan pl = plan_of(a, Nk);
+        const StepPlan pl = plan_of(a, false, Nk);
         MBR_CHECK(pl.bytes == 0 || (workspace && workspace_bytes >= pl.bytes), "window_attention: workspace too small");
         attend_step(a, dtype, false, false, pl, workspace, st);
         return;
@@ -143,7 +143,7 @@ int64_t cache_attention_workspace(const mbr_kv_cache& c, int64_t tokens, int Hq,
     const mbr_view none{};
     AttnArgs a = common_args(none, none, c.seqs, tokens, Hq, c.kv_heads, c.dim_head, left, right, c.sinks, 0.f, nullptr);
     if (c.seqs == 0 || tokens == 0 || Hq == 0 || c.dtype == DT_F32) return 0;
-    return plan_of(a, (int64_t)c.sinks + c.ring).bytes;
+    return plan_of(a, c.bits == 4, (int64_t)c.sinks + c.ring).bytes;
 }
 
 void cache_attention(const mbr_view& q, const mbr_kv_cache& c, const mbr_view& out, const int32_t* length,
@@ -157,7 +157,7 @@ void cache_attention(const mbr_view& q, const mbr_kv_cache& c, const mbr_view& o
     a.ring = c.ring, a.cache_sinks = c.sinks, a.slots = (int64_t)c.sinks + c.ring;
     a.kv_len = length;
     if (step_supported(a, c.dtype, true)) {
-        const StepPlan pl = plan_of(a, a.slots);
+        const StepPlan pl = plan_of(a, q4, a.slots);
         MBR_CHECK(pl.bytes == 0 || (workspace && workspace_bytes >= pl.bytes), "cache_attention: workspace too small");
         attend_step(a, c.dtype, true, q4, pl, workspace, st);
         return;

@@ -42,14 +42,16 @@ using namespace sm100;
 
 constexpr int UNIT = 32;  // keys a warp works on at a time
 
-// A warp's ring: SLOTS times the rows of one unit's keys or values (and, 4
-// bits, their steps and offsets).
+// A warp's ring: SLOTS times the rows of KEYS keys or values (and, 4 bits, their
+// steps and offsets): one unit of 16-bit rows, two of codes, whose copies are
+// short.
 template <int DP, bool Q4>
 struct StepCfg {
-    static constexpr int WARPS = step_warps(DP);
+    static constexpr int WARPS = step_warps(DP, Q4);
     static constexpr int ROW = Q4 ? DP / 2 : DP * 2;  // most bytes of a row
     static constexpr int SROW = Q4 ? DP / kGroup * 4 : 0;
-    static constexpr int SLOT = UNIT * (ROW + SROW);
+    static constexpr int SUBS = Q4 ? 2 : 1, KEYS = UNIT * SUBS;
+    static constexpr int SLOT = KEYS * (ROW + SROW);
     static constexpr int BUDGET = 200 * 1024 / WARPS;
     static constexpr int SLOTS = BUDGET / SLOT < 8 ? BUDGET / SLOT : 8;
     static_assert(SLOTS >= 3, "two copies in flight while one is read");
@@ -249,7 +251,7 @@ __global__ void __launch_bounds__(StepCfg<DP, Q4>::WARPS * 32, 1) attend_step_ke
     constexpr int KS = DP / 16;  // contraction steps of S
     constexpr int NT = DP / 8;   // channel tiles of O
     using Cfg = StepCfg<DP, Q4>;
-    constexpr int ROWS = HALF ? 8 : 16, SLOTS = Cfg::SLOTS, JT = UNIT / 8;
+    constexpr int ROWS = HALF ? 8 : 16, SLOTS = Cfg::SLOTS, KEYS = Cfg::KEYS, JT = UNIT / 8;
     extern __shared__ __align__(128) uint8_t smem[];
     const AttnArgs& a = p.a;
     const int D = EX ? DP : a.D;
@@ -284,7 +286,7 @@ __global__ void __launch_bounds__(StepCfg<DP, Q4>::WARPS * 32, 1) attend_step_ke
         const int rows = min(ROWS, a.Nq * a.G - r0);
         const TileKeys tk = tile_keys<CACHED>(a, s, r0, rows);
         const int total = tk.total, ns = tk.ns;
-        const int units = (total + UNIT - 1) / UNIT;
+        const int units = (total + KEYS - 1) / KEYS;  // of copies
         // this CTA's units (units / outer, the first units % outer shares one more), of which the group's warps
         // take every inner-th: they read neighbouring rows at about the same time
         const int each = (int)p.by_outer.div(units), more = units - each * p.outer;
@@ -302,7 +304,7 @@ __global__ void __launch_bounds__(StepCfg<DP, Q4>::WARPS * 32, 1) attend_step_ke
         // the n-th copy of this part (unit n / 2: keys, then values; none past the end) into a slot of the ring
         const int copies = 2 * mine;
         const int64_t s0 = s * p.s_seq + hk * p.s_head;
-        // units [run_lo, run_hi) lie whole in one run of cache rows; unit c's keys start at run_k + c * UNIT * rb
+        // units [run_lo, run_hi) lie whole in one run of cache rows; unit c's keys start at run_k + c * KEYS * rb
         int run_lo = 0, run_hi = 0;
         const uint8_t *run_k = nullptr, *run_v = nullptr;
         auto fetch = [&](int n, int to_slot) {
@@ -313,10 +315,10 @@ __global__ void __launch_bounds__(StepCfg<DP, Q4>::WARPS * 32, 1) attend_step_ke
                     if (lane == 0) {
                         const uint32_t b = bar + to_slot * 8;
                         if (c >= run_lo && c < run_hi) {
-                            expect_bytes(b, UNIT * rb);
-                            bulk_load(dst, (n & 1 ? run_v : run_k) + (int64_t)c * (UNIT * rb), UNIT * rb, b);
+                            expect_bytes(b, KEYS * rb);
+                            bulk_load(dst, (n & 1 ? run_v : run_k) + (int64_t)c * (KEYS * rb), KEYS * rb, b);
                         } else {  // the first tokens, the ring's end, its start, the last unit: run by run
-                            const int u0 = c * UNIT, u1 = min(u0 + UNIT, total);
+                            const int u0 = c * KEYS, u1 = min(u0 + KEYS, total);
                             expect_bytes(b, (uint32_t)((u1 - u0) * rb));
                             int to = 0;
                             for (int u = u0; u < u1; u = to) {
@@ -325,13 +327,13 @@ __global__ void __launch_bounds__(StepCfg<DP, Q4>::WARPS * 32, 1) attend_step_ke
                                 const int64_t at = slot(u);
                                 bulk_load(dst + (u - u0) * rb, (n & 1 ? vb0 : kb0) + at * rb, (uint32_t)((to - u) * rb), b);
                                 // the run that this unit ends in
-                                run_lo = c + 1, run_hi = end / UNIT;
+                                run_lo = c + 1, run_hi = end / KEYS;
                                 run_k = kb0 + (at - u) * rb, run_v = vb0 + (at - u) * rb;
                             }
                         }
                     }
                 } else {  // rows apart: 16-byte copies, neighbouring lanes on one row
-                    const int per = rb >> 4, u0 = c * UNIT, u1 = min(u0 + UNIT, total);
+                    const int per = rb >> 4, u0 = c * KEYS, u1 = min(u0 + KEYS, total);
                     const int64_t tok = n & 1 ? p.v_tok : p.k_tok;
                     const uint8_t* src = n & 1 ? vb0 : kb0;
                     for (int j = lane; j < (u1 - u0) * per; j += 32) {
@@ -341,13 +343,17 @@ __global__ void __launch_bounds__(StepCfg<DP, Q4>::WARPS * 32, 1) attend_step_ke
                 }
                 if constexpr (Q4) {
                     constexpr int SC = EX ? Cfg::SROW : 4;  // bytes a copy
-                    const int u = c * UNIT + lane;
-                    if (u < total) {
-                        const uint32_t d = dst + UNIT * Cfg::ROW + lane * sb;
-                        const uint8_t* x = (const uint8_t*)(n & 1 ? a.v_scale : a.k_scale) + s0 + slot(u) * sb;
+                    const uint8_t* scales = (const uint8_t*)(n & 1 ? a.v_scale : a.k_scale) + s0;
 #pragma unroll
-                        for (int e = 0; e < Cfg::SROW / SC; ++e)
-                            if (SC * e < sb) copy_async<SC>(d + SC * e, x + SC * e);
+                    for (int k = lane; k < KEYS; k += 32) {
+                        const int u = c * KEYS + k;
+                        if (u < total) {
+                            const uint32_t d = dst + KEYS * Cfg::ROW + k * sb;
+                            const uint8_t* x = scales + slot(u) * sb;
+#pragma unroll
+                            for (int e = 0; e < Cfg::SROW / SC; ++e)
+                                if (SC * e < sb) copy_async<SC>(d + SC * e, x + SC * e);
+                        }
                     }
                 }
             }
@@ -356,7 +362,7 @@ __global__ void __launch_bounds__(StepCfg<DP, Q4>::WARPS * 32, 1) attend_step_ke
         // the slot to be read next has landed
         auto landed = [&] {
             if (CACHED) wait_bytes(bar + st * 8, parity, p.err);
-            if (Q4 || !CACHED) cp_async_wait<SLOTS - 1>();
+            if (!CACHED) cp_async_wait<SLOTS - 1>();
             __syncwarp();
         };
         auto next = [&] {
@@ -415,184 +421,206 @@ __global__ void __launch_bounds__(StepCfg<DP, Q4>::WARPS * 32, 1) attend_step_ke
         float ma = -INFINITY, mb = -INFINITY, la = 0.f, lb = 0.f;  // rows g and g + 8: offset (log2 units), sum
 
         for (int n = 0; n < copies; n += 2) {
+            // 16-bit rows: the keys' slot is refilled as soon as S is computed.  Codes: both slots serve two units.
             fetch(n + SLOTS - 1, after(st, SLOTS - 1));  // into the slot read last, while this one is worked on
             landed();
-            const uint32_t kp = ring + st * Cfg::SLOT + g * rb + (Q4 ? DP / 8 * t : 16 * t);
-            const uint32_t ksp = ring + st * Cfg::SLOT + UNIT * Cfg::ROW + g * sb + DP / 4 * t / kGroup * 4;
-            const int u0 = (c0 + ((n >> 1) << p.inner_log2)) * UNIT;
-            const bool full = u0 >= full_lo && u0 + UNIT <= full_hi;  // every row sees every key
-            // ---- S = Q K^T: key tile j holds keys 8j + g ----
-            float sc[JT][4];
-            uint32_t kx[JT][Q4 ? DP / 32 : DP / 8], sm[JT];
-#pragma unroll
-            for (int j = 0; j < JT; ++j) {
-                sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
-                const uint32_t row = kp + 8 * j * rb;
-                sm[j] = 0u;
-                if constexpr (Q4) {
-#pragma unroll
-                    for (int w = 0; w < DP / 32; ++w) kx[j][w] = 0u;
-                    if (EX || DP / 4 * t < D) {
-                        load_words<DP / 8>(kx[j], row);
-                        load_words<4>(&sm[j], ksp + 8 * j * sb);
-                    }
-                } else {
-#pragma unroll
-                    for (int w = 0; w < KS / 2; ++w) {
-                        kx[j][4 * w] = kx[j][4 * w + 1] = kx[j][4 * w + 2] = kx[j][4 * w + 3] = 0u;
-                        if (EX || 32 * w + 8 * t < D) load_words<16>(kx[j] + 4 * w, row + 64 * w);
-                    }
-                }
+            const uint32_t k_slot = ring + st * Cfg::SLOT;
+            uint32_t v_slot = 0;
+            if constexpr (Q4) {
+                next();
+                wait_bytes(bar + st * 8, parity, p.err);
+                cp_async_wait<SLOTS - 2>();  // both slots' steps and offsets
+                __syncwarp();
+                v_slot = ring + st * Cfg::SLOT;
             }
-            // the key tiles' sums advance together: a product waits for the one before it on its tile only
-#pragma unroll
-            for (int w = 0; w < KS / 2; ++w)
-#pragma unroll
-                for (int half = 0; half < 2; ++half)
-#pragma unroll
-                    for (int j = 0; j < JT; ++j) {
-                        if constexpr (Q4) {
-                            const uint32_t step = __byte_perm(sm[j], 0, 0x1010), off = __byte_perm(sm[j], 0, 0x3232);
-                            mma16816(sc[j], q[2 * w + half], widen(kx[j][w], 2 * half, step, off, wd),
-                                     widen(kx[j][w], 2 * half + 1, step, off, wd), (T*)nullptr);
-                        } else {
-                            mma16816(sc[j], q[2 * w + half], kx[j][4 * w + 2 * half], kx[j][4 * w + 2 * half + 1],
-                                     (T*)nullptr);
+#pragma unroll 1
+            for (int sub = 0; sub < Cfg::SUBS; ++sub) {
+                const int u0 = (c0 + ((n >> 1) << p.inner_log2)) * KEYS + sub * UNIT;
+                if (Q4 && u0 >= total) break;
+                const uint32_t kp = k_slot + (sub * UNIT + g) * rb + (Q4 ? DP / 8 * t : 16 * t);
+                const uint32_t ksp = k_slot + KEYS * Cfg::ROW + (sub * UNIT + g) * sb + DP / 4 * t / kGroup * 4;
+                const bool full = u0 >= full_lo && u0 + UNIT <= full_hi;  // every row sees every key
+                // ---- S = Q K^T: key tile j holds keys 8j + g ----
+                float sc[JT][4];
+                uint32_t kx[JT][Q4 ? DP / 32 : DP / 8], sm[JT];
+    #pragma unroll
+                for (int j = 0; j < JT; ++j) {
+                    sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
+                    const uint32_t row = kp + 8 * j * rb;
+                    sm[j] = 0u;
+                    if constexpr (Q4) {
+    #pragma unroll
+                        for (int w = 0; w < DP / 32; ++w) kx[j][w] = 0u;
+                        if (EX || DP / 4 * t < D) {
+                            load_words<DP / 8>(kx[j], row);
+                            load_words<4>(&sm[j], ksp + 8 * j * sb);
+                        }
+                    } else {
+    #pragma unroll
+                        for (int w = 0; w < KS / 2; ++w) {
+                            kx[j][4 * w] = kx[j][4 * w + 1] = kx[j][4 * w + 2] = kx[j][4 * w + 3] = 0u;
+                            if (EX || 32 * w + 8 * t < D) load_words<16>(kx[j] + 4 * w, row + 64 * w);
                         }
                     }
-            next();
-            fetch(n + SLOTS, after(st, SLOTS - 1));
-            if (!full) {  // unseen keys get -inf
-#pragma unroll
-                for (int j = 0; j < JT; ++j)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int u = u0 + 8 * j + 2 * t + e;
-                        if (!(u < ka.f || (u >= ka.a && u < ka.b))) sc[j][e] = -INFINITY;
-                        if (!HALF && !(u < kb.f || (u >= kb.a && u < kb.b))) sc[j][2 + e] = -INFINITY;
-                    }
-            }
-            // ---- weights 2^(s - m) with the offset m so far; the sum tells (inf and
-            // NaN too) when the offset has become too low: then m becomes the
-            // maximum, what was summed is scaled, and the weights are taken again.
-            // The sum holds the weights before their rounding to the values' type.
-            uint32_t pr[JT][2];  // [key tile][row half]
-            auto weights = [&](float& ra, float& rb_) {
-                const float oa = ma == -INFINITY ? 0.f : ma, ob = mb == -INFINITY ? 0.f : mb;
-                ra = rb_ = 0.f;
-#pragma unroll
-                for (int j = 0; j < JT; ++j) {
-                    const float e0 = ex2_approx(fmaf(sc[j][0], scale, -oa)), e1 = ex2_approx(fmaf(sc[j][1], scale, -oa));
-                    ra += e0 + e1;
-                    pr[j][0] = pack2(e0, e1, (T*)nullptr);
-                    if constexpr (HALF) {
-                        pr[j][1] = 0u;
-                    } else {
-                        const float e2 = ex2_approx(fmaf(sc[j][2], scale, -ob)),
-                                    e3 = ex2_approx(fmaf(sc[j][3], scale, -ob));
-                        rb_ += e2 + e3;
-                        pr[j][1] = pack2(e2, e3, (T*)nullptr);
-                    }
                 }
-            };
-            float ra, rbs;
-            weights(ra, rbs);
-            constexpr float kMost = 256.f;
-            bool low = !(ra <= kMost) || ma == -INFINITY;
-            if constexpr (!HALF) low |= !(rbs <= kMost) || mb == -INFINITY;
-            if (__any_sync(0xffffffffu, low)) {
-                auto row_max = [&](int e) {
-                    float r = -INFINITY;
-#pragma unroll
-                    for (int j = 0; j < JT; ++j) r = fmaxf(r, fmaxf(sc[j][e], sc[j][e + 1]));
-                    r = fmaxf(r, __shfl_xor_sync(0xffffffffu, r, 1));
-                    return fmaxf(r, __shfl_xor_sync(0xffffffffu, r, 2)) * scale;
+                // the key tiles' sums advance together: a product waits for the one before it on its tile only
+    #pragma unroll
+                for (int w = 0; w < KS / 2; ++w)
+    #pragma unroll
+                    for (int half = 0; half < 2; ++half)
+    #pragma unroll
+                        for (int j = 0; j < JT; ++j) {
+                            if constexpr (Q4) {
+                                const uint32_t step = __byte_perm(sm[j], 0, 0x1010),
+                                               off = __byte_perm(sm[j], 0, 0x3232);
+                                mma16816(sc[j], q[2 * w + half], widen(kx[j][w], 2 * half, step, off, wd),
+                                         widen(kx[j][w], 2 * half + 1, step, off, wd), (T*)nullptr);
+                            } else {
+                                mma16816(sc[j], q[2 * w + half], kx[j][4 * w + 2 * half], kx[j][4 * w + 2 * half + 1],
+                                         (T*)nullptr);
+                            }
+                        }
+                if constexpr (!Q4) {
+                    next();
+                    fetch(n + SLOTS, after(st, SLOTS - 1));
+                }
+                if (!full) {  // unseen keys get -inf
+    #pragma unroll
+                    for (int j = 0; j < JT; ++j)
+    #pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const int u = u0 + 8 * j + 2 * t + e;
+                            if (!(u < ka.f || (u >= ka.a && u < ka.b))) sc[j][e] = -INFINITY;
+                            if (!HALF && !(u < kb.f || (u >= kb.a && u < kb.b))) sc[j][2 + e] = -INFINITY;
+                        }
+                }
+                // ---- weights 2^(s - m) with the offset m so far; the sum tells (inf and
+                // NaN too) when the offset has become too low: then m becomes the
+                // maximum, what was summed is scaled, and the weights are taken again.
+                // The sum holds the weights before their rounding to the values' type.
+                uint32_t pr[JT][2];  // [key tile][row half]
+                auto weights = [&](float& ra, float& rb_) {
+                    const float oa = ma == -INFINITY ? 0.f : ma, ob = mb == -INFINITY ? 0.f : mb;
+                    ra = rb_ = 0.f;
+    #pragma unroll
+                    for (int j = 0; j < JT; ++j) {
+                        const float e0 = ex2_approx(fmaf(sc[j][0], scale, -oa)),
+                                    e1 = ex2_approx(fmaf(sc[j][1], scale, -oa));
+                        ra += e0 + e1;
+                        pr[j][0] = pack2(e0, e1, (T*)nullptr);
+                        if constexpr (HALF) {
+                            pr[j][1] = 0u;
+                        } else {
+                            const float e2 = ex2_approx(fmaf(sc[j][2], scale, -ob)),
+                                        e3 = ex2_approx(fmaf(sc[j][3], scale, -ob));
+                            rb_ += e2 + e3;
+                            pr[j][1] = pack2(e2, e3, (T*)nullptr);
+                        }
+                    }
                 };
-                auto raise = [&](float& mx, float& l, int e) {
-                    const float now = fmaxf(mx, row_max(e));
-                    const float f = now == mx ? 1.f : ex2_approx(mx - now);
-                    mx = now;
-                    l *= f;
-#pragma unroll
-                    for (int i = 0; i < NT; ++i) o[i][e] *= f, o[i][e + 1] *= f;
-                };
-                raise(ma, la, 0);
-                if constexpr (!HALF) raise(mb, lb, 2);
+                float ra, rbs;
                 weights(ra, rbs);
-            }
-            la += ra;
-            lb += rbs;
-            landed();
-            const uint32_t vp = ring + st * Cfg::SLOT + 2 * t * rb + (Q4 ? DP / 16 : DP / 4) * g;
-            const uint32_t vsp = ring + st * Cfg::SLOT + UNIT * Cfg::ROW + 2 * t * sb + DP / 8 * g / kGroup * 4;
-            // ---- O += P V, 16 keys at a time: values 2t, 2t + 1, 8 + 2t, 9 + 2t ----
-#pragma unroll
-            for (int h = 0; h < UNIT / 16; ++h) {
-                const uint32_t pa[4] = {pr[2 * h][0], pr[2 * h][1], pr[2 * h + 1][0], pr[2 * h + 1][1]};
-                constexpr int W = Q4 ? (DP + 63) / 64 : DP / 16;
-                uint32_t v[4][W], vs[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int kr = 16 * h + 8 * (j >> 1) + (j & 1);
-                    const uint32_t row = vp + kr * rb;
-                    if constexpr (!EX) {
-#pragma unroll
-                        for (int w = 0; w < W; ++w) v[j][w] = 0u;
-                        vs[j] = 0u;
+                constexpr float kMost = 256.f;
+                bool low = !(ra <= kMost) || ma == -INFINITY;
+                if constexpr (!HALF) low |= !(rbs <= kMost) || mb == -INFINITY;
+                if (__any_sync(0xffffffffu, low)) {
+                    auto row_max = [&](int e) {
+                        float r = -INFINITY;
+    #pragma unroll
+                        for (int j = 0; j < JT; ++j) r = fmaxf(r, fmaxf(sc[j][e], sc[j][e + 1]));
+                        r = fmaxf(r, __shfl_xor_sync(0xffffffffu, r, 1));
+                        return fmaxf(r, __shfl_xor_sync(0xffffffffu, r, 2)) * scale;
+                    };
+                    auto raise = [&](float& mx, float& l, int e) {
+                        const float now = fmaxf(mx, row_max(e));
+                        const float f = now == mx ? 1.f : ex2_approx(mx - now);
+                        mx = now;
+                        l *= f;
+    #pragma unroll
+                        for (int i = 0; i < NT; ++i) o[i][e] *= f, o[i][e + 1] *= f;
+                    };
+                    raise(ma, la, 0);
+                    if constexpr (!HALF) raise(mb, lb, 2);
+                    weights(ra, rbs);
+                }
+                la += ra;
+                lb += rbs;
+                if constexpr (!Q4) {
+                    landed();
+                    v_slot = ring + st * Cfg::SLOT;
+                }
+                const uint32_t vp = v_slot + (sub * UNIT + 2 * t) * rb + (Q4 ? DP / 16 : DP / 4) * g;
+                const uint32_t vsp = v_slot + KEYS * Cfg::ROW + (sub * UNIT + 2 * t) * sb + DP / 8 * g / kGroup * 4;
+                // ---- O += P V, 16 keys at a time: values 2t, 2t + 1, 8 + 2t, 9 + 2t ----
+    #pragma unroll
+                for (int h = 0; h < UNIT / 16; ++h) {
+                    const uint32_t pa[4] = {pr[2 * h][0], pr[2 * h][1], pr[2 * h + 1][0], pr[2 * h + 1][1]};
+                    constexpr int W = Q4 ? (DP + 63) / 64 : DP / 16;
+                    uint32_t v[4][W], vs[4];
+    #pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int kr = 16 * h + 8 * (j >> 1) + (j & 1);
+                        const uint32_t row = vp + kr * rb;
+                        if constexpr (!EX) {
+    #pragma unroll
+                            for (int w = 0; w < W; ++w) v[j][w] = 0u;
+                            vs[j] = 0u;
+                        }
+                        if constexpr (Q4) {
+                            if (EX || DP / 8 * g < D) {
+                                load_words<DP / 16>(v[j], row);
+                                load_words<4>(&vs[j], vsp + kr * sb);
+                            }
+                        } else if constexpr (DP == 32) {
+                            if (EX || 4 * g < D) load_words<8>(v[j], row);
+                        } else {
+    #pragma unroll
+                            for (int w = 0; w < DP / 64; ++w)
+                                if (EX || DP / 8 * g + 8 * w < D) load_words<16>(v[j] + 4 * w, row + 16 * w);
+                        }
+                    }
+                    if (!full) {  // rows past the last key hold anything: zeros instead (4 bits: by step and offset)
+    #pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const bool on = u0 + 16 * h + 2 * t + 8 * (j >> 1) + (j & 1) < total;
+                            if constexpr (Q4) {
+                                vs[j] = on ? vs[j] : 0u;
+                            } else {
+    #pragma unroll
+                                for (int w = 0; w < W; ++w) v[j][w] = on ? v[j][w] : 0u;
+                            }
+                        }
                     }
                     if constexpr (Q4) {
-                        if (EX || DP / 8 * g < D) {
-                            load_words<DP / 16>(v[j], row);
-                            load_words<4>(&vs[j], vsp + kr * sb);
+                        uint32_t step[2], off[2];  // (key 2t, key 2t + 1) of each half
+    #pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            step[j] = __byte_perm(vs[2 * j], vs[2 * j + 1], 0x5410);
+                            off[j] = __byte_perm(vs[2 * j], vs[2 * j + 1], 0x7632);
                         }
-                    } else if constexpr (DP == 32) {
-                        if (EX || 4 * g < D) load_words<8>(v[j], row);
+    #pragma unroll
+                        for (int w = 0; w < NT / 4; ++w) {  // four channels at a time
+                            const uint32_t sel = (w & 1) ? 0x7632 : 0x5410;
+                            const uint32_t lo = __byte_perm(v[0][w >> 1], v[1][w >> 1], sel);
+                            const uint32_t hi = __byte_perm(v[2][w >> 1], v[3][w >> 1], sel);
+    #pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                mma16816(o[4 * w + i], pa, widen(lo, i, step[0], off[0], wd),
+                                         widen(hi, i, step[1], off[1], wd), (T*)nullptr);
+                        }
                     } else {
-#pragma unroll
-                        for (int w = 0; w < DP / 64; ++w)
-                            if (EX || DP / 8 * g + 8 * w < D) load_words<16>(v[j] + 4 * w, row + 16 * w);
-                    }
-                }
-                if (!full) {  // rows past the last key hold anything: zeros instead (4 bits: by step and offset)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const bool on = u0 + 16 * h + 2 * t + 8 * (j >> 1) + (j & 1) < total;
-                        if constexpr (Q4) {
-                            vs[j] = on ? vs[j] : 0u;
-                        } else {
-#pragma unroll
-                            for (int w = 0; w < W; ++w) v[j][w] = on ? v[j][w] : 0u;
+    #pragma unroll
+                        for (int w = 0; w < NT / 2; ++w) {
+                            mma16816(o[2 * w], pa, __byte_perm(v[0][w], v[1][w], 0x5410),
+                                     __byte_perm(v[2][w], v[3][w], 0x5410), (T*)nullptr);
+                            mma16816(o[2 * w + 1], pa, __byte_perm(v[0][w], v[1][w], 0x7632),
+                                     __byte_perm(v[2][w], v[3][w], 0x7632), (T*)nullptr);
                         }
-                    }
-                }
-                if constexpr (Q4) {
-                    uint32_t step[2], off[2];  // (key 2t, key 2t + 1) of each half
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        step[j] = __byte_perm(vs[2 * j], vs[2 * j + 1], 0x5410);
-                        off[j] = __byte_perm(vs[2 * j], vs[2 * j + 1], 0x7632);
-                    }
-#pragma unroll
-                    for (int w = 0; w < NT / 4; ++w) {  // four channels at a time
-                        const uint32_t sel = (w & 1) ? 0x7632 : 0x5410;
-                        const uint32_t lo = __byte_perm(v[0][w >> 1], v[1][w >> 1], sel);
-                        const uint32_t hi = __byte_perm(v[2][w >> 1], v[3][w >> 1], sel);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            mma16816(o[4 * w + i], pa, widen(lo, i, step[0], off[0], wd),
-                                     widen(hi, i, step[1], off[1], wd), (T*)nullptr);
-                    }
-                } else {
-#pragma unroll
-                    for (int w = 0; w < NT / 2; ++w) {
-                        mma16816(o[2 * w], pa, __byte_perm(v[0][w], v[1][w], 0x5410),
-                                 __byte_perm(v[2][w], v[3][w], 0x5410), (T*)nullptr);
-                        mma16816(o[2 * w + 1], pa, __byte_perm(v[0][w], v[1][w], 0x7632),
-                                 __byte_perm(v[2][w], v[3][w], 0x7632), (T*)nullptr);
                     }
                 }
             }
             next();
+            if constexpr (Q4) fetch(n + SLOTS, after(st, SLOTS - 2));  // the keys' slot, read with the values'
         }
 
         // ---- this part's result; accumulator column 2t, 2t + 1 of tile i is channel NT * 2t + i, NT * (2t + 1) + i ----
@@ -738,14 +766,15 @@ bool step_supported(const AttnArgs& a, int dtype, bool cached) {
     return (((uintptr_t)a.k | (uintptr_t)a.v) & 15) == 0 && all % 8 == 0;
 }
 
-StepPlan step_plan(int64_t seqs, int64_t tokens, int Hq, int Hkv, int D, int64_t keys) {
+StepPlan step_plan(int64_t seqs, int64_t tokens, int Hq, int Hkv, int D, bool q4, int64_t keys) {
     StepPlan pl{};
     const int64_t rows = tokens * (Hq / Hkv);
     pl.half = rows <= 8;
     pl.rows = (int)std::min<int64_t>(rows, 16);
     pl.tiles = ceil_div(rows, 16);
     pl.items = seqs * Hkv * pl.tiles;
-    const int dp = D == 32 ? 32 : D == 64 ? 64 : 128, warps = step_warps(dp);
+    const int dp = D == 32 ? 32 : D == 64 ? 64 : 128, warps = step_warps(dp, q4);
+    const int64_t copy = UNIT * (q4 ? 2 : 1);  // keys a warp fetches at a time
     // A warp's time is its rounds x (its keys + a start and a join worth some 100
     // keys).  One CTA an item joins inside; more CTAs cost a second kernel (some
     // 500 keys) and the reading of each share.
@@ -756,7 +785,7 @@ StepPlan step_plan(int64_t seqs, int64_t tokens, int Hq, int Hkv, int D, int64_t
         if (cost < best) best = cost, pl.inner = inner, pl.outer = outer;
     };
     for (int n = 1; n <= warps; n *= 2) consider(n, 1);
-    for (int n = 2; n <= std::min<int64_t>(148, keys / UNIT / warps); ++n)
+    for (int n = 2; n <= std::min<int64_t>(148, keys / copy / warps); ++n)
         if (pl.items * n <= 148 * 4) consider(warps, n);
     pl.bytes = pl.outer == 1 ? 0 : pl.items * pl.outer * pl.rows * (int64_t)(dp + 2) * 4;
     return pl;

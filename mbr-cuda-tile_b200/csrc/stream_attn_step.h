@@ -16,9 +16,11 @@ struct StepPlan {
     int64_t bytes;           // workspace: the results of `outer` CTAs, which a second kernel joins (0: none)
 };
 // keys: the most keys any tile can see.
-StepPlan step_plan(int64_t seqs, int64_t tokens, int Hq, int Hkv, int D, int64_t keys);
-// Warps of a CTA (one CTA an SM) for a head size of up to dp.
-constexpr int step_warps(int dp) { return dp == 128 ? 8 : 16; }
+StepPlan step_plan(int64_t seqs, int64_t tokens, int Hq, int Hkv, int D, bool q4, int64_t keys);
+// Warps of a CTA (one CTA an SM) for a head size of up to dp.  16-bit rows need
+// bytes in flight more than warps (heads of 64: 29.5 us with 8 warps against 32
+// with 16 for a frame over 1000 keys); codes need issue slots filled.
+constexpr int step_warps(int dp, bool q4) { return q4 && dp < 128 ? 16 : 8; }
 
 struct StepArgs {
     AttnArgs a;
