@@ -9,12 +9,16 @@
 //   P = 2^(S c - m)  16 bits, over the first half of S, the A operand of
 //   O += P V         128 x D, fp32, tensor memory
 // Warps 0-3 run the softmax (thread r owns row r), warp 4 issues loads (TMA) and
-// products.  The exponential unit bounds this for heads of 64 (256 operations of
-// the tensor core an exponential, of which an SM takes 16 a clock), so what
-// counts is that some warp of every scheduler always has exponentials to take:
-// four CTAs an SM (two past 64 channels) with one S each interleave freely, and
-// one CTA's wait for its products is the others' turn.  Column chunks of 32 that no
-// row of a warp sees take no exponentials (the window's two ends).
+// products.  The exponential unit (16 a clock and SM) bounds heads of 64: 256
+// operations of the tensor core an exponential.  A row's 64 exponentials take a
+// warp some 520 clocks of that unit, its way round (S read, P written, both
+// products, S again) some 1700 more, so CTAs that interleave have to fill it: three
+// an SM with one S each (128 columns of tensor memory), two past 64 channels.  At
+// 6001 frames, 8 heads, 4 sequences, a window of 1024 + 16 keys and bf16: 99 us,
+// 470 TFLOP/s of what is seen.  Measured instead: two CTAs with two S each, a load warp and a product warp, 128 us; two
+// CTAs with blocks of 128 keys 121 us; four CTAs spill registers, twice the time.
+// Column chunks of 32 that no row of a warp sees take no exponentials (the
+// window's two ends).
 //
 // The offset m is a row's maximum of the block in which it first sees a key, and
 // is raised (O and the sum scaled, the block taken again) only when a block's
@@ -119,6 +123,14 @@ __device__ __forceinline__ uint64_t bits_between(int lo, int hi) {
     return (~0ull >> (64 - (hi - lo))) << lo;
 }
 
+// True in one lane of a converged warp, the same one each time.  The compiler knows that one lane runs what depends on
+// it, and issues from uniform registers without a loop over lanes.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t pred;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(pred));
+    return pred != 0;
+}
+
 __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int c0, int c1, int c2, int c3,
                                             uint64_t* bar) {
     asm volatile(
@@ -143,11 +155,12 @@ __global__ void __launch_bounds__(160, TileCfg<DH>::CTAS)
     uint64_t* bar_p = bar + 3;       // P written, S read (4 warps)
     uint64_t* bar_k = bar + 4;       // [NS] K stage landed
     uint64_t* bar_v = bar_k + NS;    // [NS] V stage landed
-    uint32_t* tmem_slot = (uint32_t*)(bar_v + NS);
+    uint64_t* bar_end = bar_v + NS;  // after a wait that ran out: every product done
+    uint32_t* tmem_slot = (uint32_t*)(bar_end + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 4 + 2 * NS; ++i) mbar_init(&bar[i], i == 3 ? 4 : 1);
+        for (int i = 0; i < 5 + 2 * NS; ++i) mbar_init(&bar[i], i == 3 ? 4 : 1);
         fence_barrier_init();
     }
     if (warp == 4) {
@@ -214,7 +227,7 @@ __global__ void __launch_bounds__(160, TileCfg<DH>::CTAS)
         const uint64_t dQ = sdesc_sw128(smem_u32(sm + Cfg::Q));
         const uint64_t dK = sdesc_sw128(smem_u32(sm + Cfg::K));
         const uint64_t dV = sdesc_sw128_mn(smem_u32(sm + Cfg::V));
-        const int ksteps = (p.a.D + 15) / 16;  // channels past the head size are zeros: no product for whole steps of them
+        const int ksteps = (p.a.D + 15) / 16;  // whole steps of channels past the head size (zeros) are left out
         auto issue_s = [&](int st) {  // 32 bytes a step, 16 KB (Q) or 8 KB (K) a half
             const uint64_t k0 = dK + (uint64_t)(512 * DH * st);
             if (ksteps == 4 * DH) {
@@ -239,7 +252,7 @@ __global__ void __launch_bounds__(160, TileCfg<DH>::CTAS)
         Block b[NS];  // blocks g .. g + NS - 1
 #pragma unroll
         for (int i = 0; i < NS; ++i) b[i] = next_block();
-        if (lane == 0) {
+        if (elect_one()) {
             prefetch_tensormap(&tmQ);
             prefetch_tensormap(&tmK);
             prefetch_tensormap(&tmV);
@@ -256,7 +269,7 @@ __global__ void __launch_bounds__(160, TileCfg<DH>::CTAS)
             ok = wait_all(bar_q, 0) && wait_all(&bar_k[0], 0);
             if (ok) {
                 tc_fence_after();
-                if (lane == 0) issue_s(0);
+                if (elect_one()) issue_s(0);
                 __syncwarp();
             }
         }
@@ -280,18 +293,18 @@ __global__ void __launch_bounds__(160, TileCfg<DH>::CTAS)
             ok = wait_all(bar_p, gp);
             if (!ok) break;
             tc_fence_after();
-            if (lane == 0) {
+            if (elect_one()) {
                 issue_pv(st, b[0].first);
                 if (more && !fresh) {
                     issue_s(st1);
-                } else {  // the tile's output is ready with this product; S(g) is done: a next tile's Q may take its place
+                } else {  // the tile's output is ready with this product; S(g) is done: the next Q may take Q's place
                     mma_commit(bar_o);
                     if (more) load_q(b[1]);
                 }
             }
             __syncwarp();
             const Block fresh_block = next_block();  // block g + NS
-            if (lane == 0) {
+            if (elect_one()) {
                 // S(g) done: K(g)'s stage is free.  P.V(g - 1) was issued before S(g): V(g - 1)'s stage is free, for
                 // block g - 1 + NS.
                 if (fresh_block.any) load_k(fresh_block, st);
@@ -304,7 +317,7 @@ __global__ void __launch_bounds__(160, TileCfg<DH>::CTAS)
                 if (!ok) break;
                 ++qphase;
                 tc_fence_after();
-                if (lane == 0) issue_s(st1);
+                if (elect_one()) issue_s(st1);
                 __syncwarp();
             }
 #pragma unroll
@@ -313,6 +326,12 @@ __global__ void __launch_bounds__(160, TileCfg<DH>::CTAS)
             st = st1, par = par1;
             st1 = st1 + 1 == NS ? 0 : st1 + 1;
             if (st1 == 0) par1 ^= 1;
+        }
+        if (!ok) {  // a wait ran out: what is in flight ends before the CTA does (waits with a limit, too)
+            if (elect_one()) mma_commit(bar_end);
+            wait_all(bar_end, 0);
+            for (uint32_t parity = 0; parity < 2; ++parity)  // a pending copy's phase is one of the two
+                for (int i = 0; i < 1 + 2 * NS; ++i) wait_all(i == 0 ? bar_q : bar_k + i - 1, parity);
         }
     } else {
         // ---- softmax: thread r owns row r of the tile (tensor-memory lane r) ----
@@ -397,7 +416,33 @@ __global__ void __launch_bounds__(160, TileCfg<DH>::CTAS)
                     return (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 };
                 float rs = 0.f;
-                bool low = see != 0 && m == -INFINITY;
+                bool low = see != 0 && m == -INFINITY, settled = false;
+                // The ordinary block, every row seeing all of it with an offset: straight through (the long prompt: 104
+                // us against 111 with this block in the loop below, which all others take).
+                if (whole == 3 && !__any_sync(0xffffffffu, low)) {
+                    const float mo = m == -INFINITY ? 0.f : m;
+                    const float2 mm = make_float2(-mo, -mo), cc = make_float2(c, c);
+                    float2 sum[4] = {};
+                    uint32_t s0[32], s1[32];
+                    tmem_ld32(tS, s0);
+                    tmem_ld32(tS + 32, s1);
+                    tmem_ld_wait(s0);
+                    tmem_ld_wait(s1);
+#pragma unroll
+                    for (int i = 0; i < 64; i += 2) {
+                        const uint32_t* sv = i < 32 ? s0 + i : s1 + i - 32;
+                        const float2 x2 = make_float2(__uint_as_float(sv[0]), __uint_as_float(sv[1]));
+                        const float2 z = __ffma2_rn(x2, cc, mm);
+                        const float2 e = make_float2(ex2_approx(z.x), ex2_approx(z.y));
+                        sum[i / 2 & 3] = __fadd2_rn(sum[i / 2 & 3], e);
+                        pk[i / 2] = pack2(e.x, e.y, (T*)nullptr);
+                    }
+                    const float2 all = __fadd2_rn(__fadd2_rn(sum[0], sum[1]), __fadd2_rn(sum[2], sum[3]));
+                    rs = all.x + all.y;
+                    low = sees && !(rs <= kRescaleSum);
+                    settled = !__any_sync(0xffffffffu, low);
+                }
+                if (!settled)
 #pragma unroll 1
                 for (int pass = 0; pass < 3; ++pass) {
                     if (__any_sync(0xffffffffu, low)) {
@@ -539,9 +584,9 @@ void launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, co
         MBR_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::TOTAL));
         MBR_CUDA(cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev));
     }
-    // Persistent CTAs take tiles in turn and load the next one's Q behind the last product (the 8 s chunk: 99 us against
-    // 119 with a CTA a tile).  With lengths given, what a tile holds is not known here: a CTA a tile, so that the
-    // hardware evens it out (ragged pieces: 58 us against 63).
+    // Persistent CTAs take tiles in turn and load the next one's Q behind the last product (60 x 8 heads of 801 frames:
+    // 99 us against 119 with a CTA a tile).  With lengths given, what a tile holds is not known here: a CTA a tile, so
+    // that the hardware evens it out (ragged pieces, heads of 128: 58 us against 63).
     const unsigned grid =
         p.a.q_len || p.a.kv_len ? p.ntiles : std::min<unsigned>(p.ntiles, (unsigned)(sms[dev] * Cfg::CTAS));
     kern<<<grid, 160, Cfg::TOTAL, st>>>(q, k, v, p);
