@@ -3,6 +3,7 @@
 // channels.  Both move each byte once; memory (or, for a single frame, the
 // launch) bounds them.
 #include <algorithm>
+#include <type_traits>
 
 #include "stream_cache.cuh"
 
@@ -126,11 +127,32 @@ __global__ void __launch_bounds__(256) cache_rows_kernel(const RowArgs a) {
     }
 }
 
+// Least and greatest of the 32 values that 4 lanes hold, 8 each in w; NaN where one is NaN.
+template <typename T>
+__device__ __forceinline__ float2 low_high(const uint32_t (&w)[4]) {
+    using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+    T2 x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const T2*>(&w[i]);
+    const T2 lo = __hmin2_nan(__hmin2_nan(x[0], x[1]), __hmin2_nan(x[2], x[3]));
+    const T2 hi = __hmax2_nan(__hmax2_nan(x[0], x[1]), __hmax2_nan(x[2], x[3]));
+    // (least, -greatest): one minimum for both from here on
+    T2 m;
+    m.x = __hmin_nan(lo.x, lo.y);
+    m.y = __hneg(__hmax_nan(hi.x, hi.y));
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, *reinterpret_cast<const uint32_t*>(&m), o);
+        m = __hmin2_nan(m, *reinterpret_cast<const T2*>(&other));
+    }
+    return make_float2(to_f32<T>(m.x), -to_f32<T>(m.y));
+}
+
 // Vector form: 8 channels a lane (rows on 16-byte boundaries).  A lane group takes
 // four neighbouring tokens of one head, whose cache rows lie next to each other:
 // their place is worked out once, and all eight loads are in flight before the
 // first is used.  A 4-bit group's minimum and maximum are two shuffle steps
-// (4 lanes a group).
+// (4 lanes a group), in 16 bits.
 template <typename T, bool Q4, bool READ>
 __global__ void __launch_bounds__(256) cache_vec_kernel(const RowArgs a, int lanes_log2) {
     const int D = a.c.dim_head, lanes = 1 << lanes_log2, sub = threadIdx.x & (lanes - 1);
@@ -160,6 +182,8 @@ __global__ void __launch_bounds__(256) cache_vec_kernel(const RowArgs a, int lan
                 row[u] = base + slot_of((int)p, a.c.sinks, a.c.ring);
         }
     }
+    // none of the warp's tokens stays in the cache
+    if (!READ && !__any_sync(0xffffffffu, row[0] >= 0 || row[1] >= 0 || row[2] >= 0 || row[3] >= 0)) return;
     constexpr int W = sizeof(T) / 2;  // 16-byte pieces of 8 elements
 #pragma unroll
     for (int kv = 0; kv < 2; ++kv) {
@@ -183,10 +207,15 @@ __global__ void __launch_bounds__(256) cache_vec_kernel(const RowArgs a, int lan
                 const T* f = reinterpret_cast<const T*>(&sm[u]);
                 T* e = reinterpret_cast<T*>(raw[u]);
                 const float st = to_f32<T>(f[0]), m = to_f32<T>(f[1]);
+                // codes as the low byte of 2^23 + code: no conversion
+                const uint32_t even = codes[u] & 0x0f0f0f0fu, odd = (codes[u] >> 4) & 0x0f0f0f0fu;
 #pragma unroll
-                for (int c = 0; c < 8; c += 2)
-                    store_pair<T>(e + c, make_float2(m + st * (float)((int)((codes[u] >> (4 * c)) & 15) - 8),
-                                                     m + st * (float)((int)((codes[u] >> (4 * c + 4)) & 15) - 8)));
+                for (int c = 0; c < 4; ++c) {
+                    const float2 x = make_float2(__uint_as_float(__byte_perm(even, 0x4b000000u, 0x7650 + c)),
+                                                 __uint_as_float(__byte_perm(odd, 0x4b000000u, 0x7650 + c)));
+                    const float2 q = __fadd2_rn(x, make_float2(-8388616.f, -8388616.f));
+                    store_pair<T>(e + 2 * c, __ffma2_rn(make_float2(st, st), q, make_float2(m, m)));
+                }
             }
         } else {
 #pragma unroll
@@ -199,31 +228,33 @@ __global__ void __launch_bounds__(256) cache_vec_kernel(const RowArgs a, int lan
         if constexpr (!READ && Q4) {
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const T* e = reinterpret_cast<const T*>(raw[u]);
-                float v[8], lo = INFINITY, hi = -INFINITY, odd = 0.f;
-#pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    v[c] = to_f32<T>(e[c]);
-                    lo = fminf(lo, v[c]), hi = fmaxf(hi, v[c]);
-                    odd = fmaf(v[c], 0.f, odd);  // NaN once a value is not finite
-                }
-#pragma unroll
-                for (int o = 1; o < 4; o <<= 1) {
-                    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-                    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-                    odd += __shfl_xor_sync(0xffffffffu, odd, o);
-                }
-                const bool ok = odd == 0.f && isfinite(hi - lo);
+                const uint32_t w[4] = {raw[u][0].x, raw[u][0].y, raw[u][0].z, raw[u][0].w};
+                const float2 range = low_high<T>(w);
+                const float lo = range.x, hi = range.y;
+                const bool ok = isfinite(hi - lo);  // a value that is not finite makes one of them so
                 const T sT = from_f32<T>(__fmul_rn(hi - lo, 1.f / 15.f));
                 const float st = to_f32<T>(sT);
                 const T mT = from_f32<T>(__fadd_rn(lo, 8.f * st));
                 const float m = to_f32<T>(mT), inv = st > 0.f ? __frcp_rn(st) : 0.f;
-                uint32_t codes = 0;
+                // rint((v - m) / st) + 8 within 0..15: adding 1.5 2^23 rounds to an integer; four codes are put
+                // together as one (their sum is below 2^16) in floating point
+                float part[2];
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    const float q = rintf(__fmul_rn(__fadd_rn(v[c], -m), inv)) + 8.f;
-                    codes |= (uint32_t)(int)fminf(fmaxf(q, 0.f), 15.f) << (4 * c);
+                for (int half = 0; half < 2; ++half) {
+                    float q[4];
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const T* e = reinterpret_cast<const T*>(w + 2 * half + c);
+                        const float2 d = __fadd2_rn(make_float2(to_f32<T>(e[0]), to_f32<T>(e[1])), make_float2(-m, -m));
+                        float2 x = __fmul2_rn(d, make_float2(inv, inv));
+                        x.x = fminf(fmaxf(x.x, -8.f), 7.f), x.y = fminf(fmaxf(x.y, -8.f), 7.f);
+                        x = __fadd2_rn(x, make_float2(12582920.f, 12582920.f));
+                        x = __fadd2_rn(x, make_float2(-12582912.f, -12582912.f));
+                        q[2 * c] = x.x, q[2 * c + 1] = x.y;
+                    }
+                    part[half] = fmaf(4096.f, q[3], fmaf(256.f, q[2], fmaf(16.f, q[1], q[0]))) + 8388608.f;
                 }
+                const uint32_t codes = __byte_perm(__float_as_uint(part[0]), __float_as_uint(part[1]), 0x5410);
                 if (row[u] >= 0) {
                     *reinterpret_cast<uint32_t*>(data + row[u] * (D / 2) + sub * 4) = codes;
                     if ((sub & 3) == 0) {
