@@ -99,8 +99,15 @@ AttnArgs window_args(const mbr_view& q, const mbr_view& k, const mbr_view& v, co
     return a;
 }
 
-// The form for few queries: rows that fit its tiles a few times over.
-bool few_rows(const AttnArgs& a) { return (int64_t)a.Nq * a.G <= 64; }
+// The form for few queries: it splits the keys of 16 rows at a time, where the tile
+// form takes 128 rows and all their keys.  16 rows (us, few-token form / tiles; heads
+// of 64): 60 sequences of 801 keys and 8 key heads 35 / 33, of 2 key heads 14.5 / 16,
+// 8 sequences of 4001 keys 36 / 57.  32 rows read the keys twice: 58 / 33, 21 / 16, and
+// 37 / 57 where the tiles would leave most SMs idle; 64 rows 114 / 34, 33 / 16, 64 / 57.
+bool few_rows(const AttnArgs& a) {
+    const int64_t rows = (int64_t)a.Nq * a.G;
+    return rows <= 16 || (rows <= 32 && a.seqs * a.Hkv < 148);
+}
 
 StepPlan plan_of(const AttnArgs& a, bool q4, int64_t held) {
     return step_plan(a.seqs, a.Nq, a.Hq, a.Hkv, a.D, q4, most_keys(a, held));
