@@ -11,14 +11,19 @@
 // Warps 0-3 run the softmax (thread r owns row r), warp 4 issues loads (TMA) and
 // products.  The exponential unit (16 a clock and SM) bounds heads of 64: 256
 // operations of the tensor core an exponential.  A row's 64 exponentials take a
-// warp some 520 clocks of that unit, its way round (S read, P written, both
-// products, S again) some 1700 more, so CTAs that interleave have to fill it: three
-// an SM with one S each (128 columns of tensor memory), two past 64 channels.  At
-// 6001 frames, 8 heads, 4 sequences, a window of 1024 + 16 keys and bf16: 99 us,
-// 470 TFLOP/s of what is seen.  Measured instead: two CTAs with two S each, a load warp and a product warp, 128 us; two
-// CTAs with blocks of 128 keys 121 us; four CTAs spill registers, twice the time.
-// Column chunks of 32 that no row of a warp sees take no exponentials (the
-// window's two ends).
+// warp 512 clocks of that unit, the way from P through both products to the next S
+// some 850, so CTAs that interleave have to fill it: three an SM with one S each
+// (128 columns of tensor memory; two past 64 channels), each of which then takes
+// some 2250 clocks a block, 68 % of the unit's rate.  Column chunks of 32 that no row of
+// a warp sees take no exponentials (the window's two ends).
+//
+// 6001 frames of 4 sequences x 8 heads of 64, a window of 1024 + 16 keys, bf16: 91 us,
+// 510 TFLOP/s of what is seen; 801 frames of 60 x 8 heads, 271 + 4 keys, fp16: 94 us,
+// of 30 for the bytes (a tile's start and end, and blocks that its rows see in
+// part, are much of its 7 blocks).  Measured on the first, when this took 99 us: two CTAs
+// with two S each, a load warp and a product warp 128, two CTAs with blocks of
+// 128 keys 121; four CTAs spill registers, twice the time; two Q and two stages
+// instead of three 94 where this takes 91.
 //
 // The offset m is a row's maximum of the block in which it first sees a key, and
 // is raised (O and the sum scaled, the block taken again) only when a block's
@@ -417,8 +422,8 @@ __global__ void __launch_bounds__(160, TileCfg<DH>::CTAS)
                 };
                 float rs = 0.f;
                 bool low = see != 0 && m == -INFINITY, settled = false;
-                // The ordinary block, every row seeing all of it with an offset: straight through (the long prompt: 104
-                // us against 111 with this block in the loop below, which all others take).
+                // The ordinary block, every row seeing all of it with an offset: straight through (a minute of audio:
+                // 104 us against 111 with such blocks in the loop below, which all others take).
                 if (whole == 3 && !__any_sync(0xffffffffu, low)) {
                     const float mo = m == -INFINITY ? 0.f : m;
                     const float2 mm = make_float2(-mo, -mo), cc = make_float2(c, c);
@@ -585,8 +590,8 @@ void launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, co
         MBR_CUDA(cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev));
     }
     // Persistent CTAs take tiles in turn and load the next one's Q behind the last product (60 x 8 heads of 801 frames:
-    // 99 us against 119 with a CTA a tile).  With lengths given, what a tile holds is not known here: a CTA a tile, so
-    // that the hardware evens it out (ragged pieces, heads of 128: 58 us against 63).
+    // 94 us against 116 with a CTA a tile; 4 x 8 heads of 6001: 91 against 93).  With lengths given, what a tile holds is
+    // not known here: a CTA a tile, so that the hardware evens it out (ragged pieces, heads of 128: 50 us against 55).
     const unsigned grid =
         p.a.q_len || p.a.kv_len ? p.ntiles : std::min<unsigned>(p.ntiles, (unsigned)(sms[dev] * Cfg::CTAS));
     kern<<<grid, 160, Cfg::TOTAL, st>>>(q, k, v, p);
@@ -617,9 +622,13 @@ void attend_tiles(const AttnArgs& a, int dtype, cudaStream_t st) {
     const int64_t sg = a.seqs * p.groups;
     MBR_CHECK(sg * p.qtiles < (1ll << 30), "attention: too many tiles");
     p.ntiles = (unsigned)(sg * p.qtiles);
-    // With no limit on the left, later queries see more: they go first, so that what is left at the end is small.
-    // Otherwise a sequence-head's tiles go together and find its keys in L2.
-    p.last_first = a.left < 0 && a.right >= 0;
+    // With a limit on the right the earliest queries see fewest keys.  Later ones go first, so that what is left at the
+    // end is small, where there is no limit on the left (all differ) or the tiles make few rounds (4 rounds: 91 us
+    // against 99; 8 rounds: 95 against 94).  Otherwise a sequence-head's tiles go together and find its keys in L2; six
+    // rounds of windows fit there in any order.
+    const bool wide = a.D > 64;
+    const unsigned round = 148 * (wide ? TileCfg<2>::CTAS : TileCfg<1>::CTAS);
+    p.last_first = a.right >= 0 && (a.left < 0 || p.ntiles <= 6 * round);
     p.by_inner = FastDiv(p.last_first ? (unsigned)sg : (unsigned)p.qtiles);
     p.by_groups = FastDiv((unsigned)p.groups);
     p.by_pack = FastDiv((unsigned)p.pack);
@@ -629,7 +638,6 @@ void attend_tiles(const AttnArgs& a, int dtype, cudaStream_t st) {
     make_map(&q, a.q, a.q_seq, a.q_tok, a.q_head, a.D, a.Hq, a.Nq, a.seqs, p.pack, p.tokens, dtype);
     make_map(&k, a.k, a.k_seq, a.k_tok, a.k_head, a.D, a.Hkv, a.Nk, a.seqs, 1, KB, dtype);
     make_map(&v, a.v, a.v_seq, a.v_tok, a.v_head, a.D, a.Hkv, a.Nk, a.seqs, 1, KB, dtype);
-    const bool wide = a.D > 64;
     if (dtype == DT_BF16) {
         if (wide) launch<__nv_bfloat16, 2>(q, k, v, p, st);
         else launch<__nv_bfloat16, 1>(q, k, v, p, st);
