@@ -590,8 +590,8 @@ void launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, co
         MBR_CUDA(cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev));
     }
     // Persistent CTAs take tiles in turn and load the next one's Q behind the last product (60 x 8 heads of 801 frames:
-    // 94 us against 116 with a CTA a tile; 4 x 8 heads of 6001: 91 against 93).  With lengths given, what a tile holds is
-    // not known here: a CTA a tile, so that the hardware evens it out (ragged pieces, heads of 128: 50 us against 55).
+    // 94 us against 116 with a CTA a tile; 4 x 8 heads of 6001: 91 against 93).  With lengths given, what a tile holds
+    // is not known here: a CTA a tile, so that the hardware evens it out (ragged pieces, heads of 128: 50 us against 55).
     const unsigned grid =
         p.a.q_len || p.a.kv_len ? p.ntiles : std::min<unsigned>(p.ntiles, (unsigned)(sms[dev] * Cfg::CTAS));
     kern<<<grid, 160, Cfg::TOTAL, st>>>(q, k, v, p);
