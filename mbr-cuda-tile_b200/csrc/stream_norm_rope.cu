@@ -9,7 +9,7 @@
 // of 8 + 8 heads of 64 in fp16, two axes, read in place from a packed q|k|v
 // (197 MB): 41.6 us, 4.7 TB/s (the form for any layout: 260 us); 60 tokens 2.2 us.
 // At fp32, heads of 32 and three axes the angles' loads and the instructions of
-// the turn weigh more: 51 MB in 15.7 us, 3.3 TB/s.
+// the turn weigh more: 51 MB in 14.7 us, 3.5 TB/s.
 #include <algorithm>
 
 #include "common.cuh"
@@ -231,10 +231,14 @@ void launch_steps(NormRopeArgs a, cudaStream_t st) {
 // With few tokens a step is one head a lane group (more warps share the latency),
 // otherwise four (more loads in flight a warp).  16 heads of 64 in fp16 (us, one /
 // four): 480 tokens 2.6 / 3.3, 960 tokens 3.0 / 3.4, 3840 tokens 5.8 / 5.4, 48060
-// tokens 55 / 41.
+// tokens 55 / 41.  Three where four would leave more lanes without a head: 8 + 2 heads of
+// 32 in fp32, 19980 tokens, 14.7 us against 15.7.
 template <typename T, int LANES, bool WHOLE>
 void launch_unrolled(const NormRopeArgs& a, cudaStream_t st) {
+    constexpr int GROUPS = 32 / LANES;
+    const int heads = a.Hq + a.Hkv;
     if (a.ntok * (a.Hq + a.Hkv) <= 148 * 64 * 32 / LANES) launch_steps<T, LANES, 1, WHOLE>(a, st);
+    else if (ceil_div(heads, 3 * GROUPS) * 3 < ceil_div(heads, 4 * GROUPS) * 4) launch_steps<T, LANES, 3, WHOLE>(a, st);
     else launch_steps<T, LANES, 4, WHOLE>(a, st);
 }
 template <typename T, int LANES>

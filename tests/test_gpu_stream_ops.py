@@ -70,6 +70,16 @@ def test_qk_norm_rope(torch_cuda, dtype, S, N, H, G, D, pairs):
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("S,N,H,G,D,pairs", [
+    (60, 101, 8, 2, 32, [8, 4, 4]),  # heads that do not fill a step of the form for many tokens
+    (41, 103, 8, 8, 64, [20]),       # some pairs are not turned
+    (30, 100, 9, 4, 128, [40, 24]),
+])
+def test_qk_norm_rope_many_tokens(torch_cuda, dtype, S, N, H, G, D, pairs):
+    test_qk_norm_rope(torch_cuda, dtype, S, N, H, G, D, pairs)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
 @pytest.mark.parametrize("layout", ["packed", "offset", "in_place", "no_gamma"])
 def test_qk_norm_rope_layouts(torch_cuda, dtype, layout):
     """Views of the packed q|k|v rows along the time axis, rows that are not 16-byte aligned, results in place, no gain."""
@@ -313,6 +323,20 @@ def _window_case(torch, dtype, S, N, M, H, G, D, left, right, sinks, q_len=None,
     (1, 300, 300, 1, 1, 64, 2 ** 31 - 1, 2 ** 31 - 1, 2),
 ])
 def test_window_attention(torch_cuda, dtype, S, N, M, H, G, D, left, right, sinks):
+    _window_case(torch_cuda, dtype, S, N, M, H, G, D, left, right, sinks)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("S,N,M,H,G,D,left,right,sinks", [
+    (30, 130, 150, 8, 8, 64, 70, 3, 2),   # several tiles a CTA, the latest queries first
+    (30, 140, 140, 8, 8, 32, 70, -1, 0),  # in order
+    (20, 130, 140, 8, 8, 128, -1, 0, 0),
+    (40, 150, 100, 8, 2, 64, 20, 0, 1),   # more queries than keys: the first see nothing
+    (1, 16, 90, 2, 1, 64, 30, 0, 1),      # two row tiles of the form for few queries
+    (1, 25, 300, 1, 1, 128, -1, 0, 0),
+    (100, 20, 70, 2, 2, 64, 33, 2, 0),    # as many rows, but many sequences
+])
+def test_window_attention_many_tiles(torch_cuda, dtype, S, N, M, H, G, D, left, right, sinks):
     _window_case(torch_cuda, dtype, S, N, M, H, G, D, left, right, sinks)
 
 
