@@ -144,15 +144,15 @@ def main(argv=None):
     want = whole.prompt(x)
     live = random_layer(**make)
     first = n // 2
-    got = [live.prompt(x[:first])]
+    got = [live.prompt(x[:first]), live.step(x[first:first + 1])]  # the first step loads the kernels
     start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
     start.record()
-    got += [live.step(x[i:i + 1]) for i in range(first, n)]
+    got += [live.step(x[i:i + 1]) for i in range(first + 1, n)]
     end.record()
     end.synchronize()
     err = (torch.cat(got).float() - want.float()).abs().max().item()
     print(f"{n} frames, {first} at once and the rest one by one: largest difference from one pass {err:.3e} "
-          f"(largest value {want.abs().max().item():.2f}), {start.elapsed_time(end) / (n - first):.3f} ms a frame")
+          f"(largest value {want.abs().max().item():.2f}), {start.elapsed_time(end) / max(1, n - first - 1):.3f} ms a frame")
 
 
 if __name__ == "__main__":
