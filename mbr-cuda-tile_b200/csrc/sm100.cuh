@@ -25,6 +25,8 @@ __device__ __forceinline__ bool smem_aligned_or_flag(const void* smem, int* err)
 // Upper bound on mbarrier polls before a wait is declared dead (each poll is a
 // try_wait that itself suspends for a hardware-defined interval).
 constexpr uint32_t kMaxPolls = 1u << 24;
+// ... and of a wait for copies and products still in flight once one is: these take microseconds.
+constexpr uint32_t kDrainPolls = 1u << 16;
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
@@ -65,6 +67,14 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* e
         if ((i & 1023u) == 1023u && *(volatile int*)err != KERR_NONE) return false;  // another CTA gave up
     }
     atomicExch(err, KERR_TIMEOUT);
+    return false;
+}
+
+// The same for a role that is giving up: waits for what it has in flight whatever
+// the error word says (it is set by then), 2^16 polls at most.
+__device__ __forceinline__ bool mbar_drain(uint64_t* bar, uint32_t parity) {
+    for (uint32_t i = 0; i < kDrainPolls; ++i)
+        if (mbar_try_wait(bar, parity)) return true;
     return false;
 }
 

@@ -76,9 +76,9 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 __device__ __forceinline__ void expect_bytes(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-// Waits (with a limit) for the phase of the given parity; what runs out is
-// recorded in *err and passed: the host sees the error word, the results are void.
-__device__ __forceinline__ void wait_bytes(uint32_t bar, uint32_t parity, int* err) {
+// Waits (with a limit) for the phase of the given parity.  False if it ran out (*err is set then: the host
+// sees it, the results are void).
+__device__ __forceinline__ bool wait_bytes(uint32_t bar, uint32_t parity, int* err) {
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
@@ -87,7 +87,7 @@ __device__ __forceinline__ void wait_bytes(uint32_t bar, uint32_t parity, int* e
         : "=r"(ok)
         : "r"(bar), "r"(parity)
         : "memory");
-    if (!ok) mbar_wait((uint64_t*)__cvta_shared_to_generic(bar), parity, err);
+    return ok || mbar_wait((uint64_t*)__cvta_shared_to_generic(bar), parity, err);
 }
 template <int N>
 __device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
@@ -273,6 +273,7 @@ __global__ void __launch_bounds__(StepCfg<DP, Q4>::WARPS * 32, 1) attend_step_ke
     if (p.outer > 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     int st = 0;           // slot to be read next
     uint32_t parity = 0;  // and the parity of its use
+    bool alive = true;    // false once a wait of this warp ran out: it copies and writes nothing from then on
     auto after = [](int x, int n) { return x + n >= SLOTS ? x + n - SLOTS : x + n; };
     const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;  // a negative scale turns Q's signs
     const float scale = fabsf(p.scale_log2);
@@ -297,7 +298,7 @@ __global__ void __launch_bounds__(StepCfg<DP, Q4>::WARPS * 32, 1) attend_step_ke
         const int each = (int)p.by_outer.div(units), more = units - each * p.outer;
         const int c0 = each * (int)share + min((int)share, more) + part,
                   c1 = each * (int)(share + 1) + min((int)share + 1, more);
-        const int mine = c1 > c0 ? (c1 - c0 + inner - 1) >> p.inner_log2 : 0;
+        const int mine = alive && c1 > c0 ? (c1 - c0 + inner - 1) >> p.inner_log2 : 0;
 
         // slot of key index u; a ring starts over at most once (total - ns <= ring), at index `wrap`
         const unsigned ring0 =
@@ -364,11 +365,25 @@ __global__ void __launch_bounds__(StepCfg<DP, Q4>::WARPS * 32, 1) attend_step_ke
             }
             if (Q4 || !CACHED) cp_async_commit();
         };
-        // the slot to be read next has landed
-        auto landed = [&] {
-            if (CACHED) wait_bytes(bar + st * 8, parity, p.err);
-            if (!CACHED) cp_async_wait<SLOTS - 1>();
-            __syncwarp();
+        // The slot to be read next has landed; false (in every lane) if the wait for it ran out.  Then what else this
+        // warp has in flight (the copies before the `sent`-th, one a slot) is waited for too: nothing may land in
+        // shared memory that the warp has left.
+        auto landed = [&](int n, int sent) {
+            if constexpr (CACHED) {
+                if (!__all_sync(0xffffffffu, wait_bytes(bar + st * 8, parity, p.err))) {
+                    for (int i = n; i < min(sent, copies); ++i) {
+                        const int at = after(st, i - n);
+                        mbar_drain((uint64_t*)__cvta_shared_to_generic(bar + at * 8), parity ^ (at < st));
+                    }
+                    if (Q4) cp_async_wait<0>();
+                    __syncwarp();
+                    return alive = false;
+                }
+            } else {
+                cp_async_wait<SLOTS - 1>();
+                __syncwarp();
+            }
+            return true;
         };
         auto next = [&] {
             __syncwarp();  // every lane has read the slot
@@ -428,12 +443,12 @@ __global__ void __launch_bounds__(StepCfg<DP, Q4>::WARPS * 32, 1) attend_step_ke
         for (int n = 0; n < copies; n += 2) {
             // 16-bit rows: the keys' slot is refilled as soon as S is computed.  Codes: both slots serve two units.
             fetch(n + SLOTS - 1, after(st, SLOTS - 1));  // into the slot read last, while this one is worked on
-            landed();
+            if (!landed(n, n + SLOTS)) break;
             const uint32_t k_slot = ring + st * Cfg::SLOT;
             uint32_t v_slot = 0;
             if constexpr (Q4) {
                 next();
-                wait_bytes(bar + st * 8, parity, p.err);
+                if (!landed(n + 1, n + SLOTS)) break;
                 cp_async_wait<SLOTS - 2>();  // both slots' steps and offsets
                 __syncwarp();
                 v_slot = ring + st * Cfg::SLOT;
@@ -551,7 +566,7 @@ __global__ void __launch_bounds__(StepCfg<DP, Q4>::WARPS * 32, 1) attend_step_ke
                 la += ra;
                 lb += rbs;
                 if constexpr (!Q4) {
-                    landed();
+                    if (!landed(n + 1, n + SLOTS + 1)) break;
                     v_slot = ring + st * Cfg::SLOT;
                 }
                 const uint32_t vp = v_slot + (sub * UNIT + 2 * t) * rb + (Q4 ? DP / 16 : DP / 4) * g;
@@ -624,6 +639,7 @@ __global__ void __launch_bounds__(StepCfg<DP, Q4>::WARPS * 32, 1) attend_step_ke
                     }
                 }
             }
+            if (!alive) break;
             next();
             if constexpr (Q4) fetch(n + SLOTS, after(st, SLOTS - 2));  // the keys' slot, read with the values'
         }
@@ -633,7 +649,9 @@ __global__ void __launch_bounds__(StepCfg<DP, Q4>::WARPS * 32, 1) attend_step_ke
         la += __shfl_xor_sync(0xffffffffu, la, 2);
         lb += __shfl_xor_sync(0xffffffffu, lb, 1);
         lb += __shfl_xor_sync(0xffffffffu, lb, 2);
-        // The group's results are joined through its warps' rings, whose copies have all landed and are read.
+        // The group's results are joined through its warps' rings, whose copies have all landed and are read.  (A warp
+        // whose wait ran out writes nothing there and keeps to the group's barriers: the rows are void, the error
+        // word says so.)
         constexpr int LD = DP + 2;  // a row's sums, its offset and sum
         auto put = [&](int r, int e, float m, float l) {
             float* dst = reinterpret_cast<float*>(smem + warp * Cfg::RING) + r * LD;
@@ -644,9 +662,9 @@ __global__ void __launch_bounds__(StepCfg<DP, Q4>::WARPS * 32, 1) attend_step_ke
             }
             if (t == 0) dst[DP] = m, dst[DP + 1] = l;
         };
-        if (g < rows) put(g, 0, ma, la);
+        if (alive && g < rows) put(g, 0, ma, la);
         if constexpr (!HALF) {
-            if (g + 8 < rows) put(g + 8, 2, mb, lb);
+            if (alive && g + 8 < rows) put(g + 8, 2, mb, lb);
         }
         auto group_sync = [&] {
             if (inner > 1) asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(inner * 32) : "memory");
