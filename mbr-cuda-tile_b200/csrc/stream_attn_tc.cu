@@ -334,9 +334,11 @@ __global__ void __launch_bounds__(160, TileCfg<DH>::CTAS)
         }
         if (!ok) {  // a wait ran out: what is in flight ends before the CTA does (waits with a limit, too)
             if (elect_one()) mma_commit(bar_end);
-            wait_all(bar_end, 0);
+            __syncwarp();
+            mbar_drain(bar_end, 0);
             for (uint32_t parity = 0; parity < 2; ++parity)  // a pending copy's phase is one of the two
-                for (int i = 0; i < 1 + 2 * NS; ++i) wait_all(i == 0 ? bar_q : bar_k + i - 1, parity);
+                for (int i = 0; i < 1 + 2 * NS; ++i) mbar_drain(i == 0 ? bar_q : bar_k + i - 1, parity);
+            __syncwarp();
         }
     } else {
         // ---- softmax: thread r owns row r of the tile (tensor-memory lane r) ----
@@ -535,6 +537,9 @@ __global__ void __launch_bounds__(160, TileCfg<DH>::CTAS)
                 attend_row<T, false, false>(a, x.s, x.tok0 + qt, x.h0 + q - qt * p.pack, x.n, x.m);
             }
         }
+        // a wait ran out: the tile's last product, if it was issued, ends before the CTA does
+        if (!ok) mbar_drain(bar_o, tiles & 1);
+        __syncwarp();
     }
     tc_fence_before();
     __syncthreads();

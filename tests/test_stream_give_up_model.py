@@ -1,4 +1,5 @@
-"""CPU model of what the streaming attention's few-token kernel (csrc/stream_attn_step.cu) does when a wait runs out: whichever wait it is and whatever has landed by then, no copy is started into a slot that one is
+"""CPU models of what the streaming attention kernels do when a wait runs out (csrc/stream_attn_step.cu,
+csrc/stream_attn_tc.cu): whichever wait it is and whatever has landed by then, no copy is started into a slot that one is
 still on its way to, nothing is written over a slot that a copy is on its way to, no warp leaves the others at a barrier, and
 no copy or product is in flight when the CTA ends.
 
@@ -133,6 +134,102 @@ def test_step_model_shows_mistakes(mistake):
     for seed in range(600):
         try:
             step_group([14], 8, False, seed, 0.3, **{mistake: True})
+        except (Fault, AssertionError):
+            n += 1
+    assert n > 0
+
+
+def tiles(blocks, ns, seed, tired, warps=2, hasty=False, leaves=False):
+    """A CTA of the tile kernel; blocks: key blocks of each of its tiles.  hasty: drains do not wait; leaves: a softmax
+    warp that gives up does not wait for its tile's last product."""
+    cta = Cta(seed, tired)
+    stream = [j == 0 for n in blocks for j in range(n)]
+    total = len(stream)
+    bar_q, bar_s, bar_o, bar_p, bar_end = Barrier(), Barrier(), Barrier(), Barrier(warps), Barrier()
+    bar_k, bar_v = [Barrier() for _ in range(ns)], [Barrier() for _ in range(ns)]
+    busy = set()
+
+    def load(name, g, bar):
+        if g < total:
+            cta.load(busy, (name, g % ns if name != "q" else 0), bar)
+
+    def issuer():
+        if not total:
+            return
+        load("q", 0, bar_q)
+        for g in range(ns):
+            load("k", g, bar_k[g % ns])
+            load("v", g, bar_v[g % ns])
+        ok = (yield from cta.wait(bar_q, 0)) and (yield from cta.wait(bar_k[0], 0))
+        if ok:
+            cta.pipe.append(bar_s.arrive)
+        q_phase, g = 1, 0
+        while ok and g < total:
+            more, fresh = g + 1 < total, g + 1 < total and stream[g + 1]
+            ok = yield from cta.wait(bar_v[g % ns], g // ns & 1)
+            if ok and more:
+                ok = yield from cta.wait(bar_k[(g + 1) % ns], (g + 1) // ns & 1)
+            ok = ok and (yield from cta.wait(bar_p, g & 1))
+            if not ok:
+                break
+            cta.pipe.append(lambda: None)  # P V
+            if more and not fresh:
+                cta.pipe.append(bar_s.arrive)
+            else:
+                cta.pipe.append(bar_o.arrive)
+                if more:
+                    load("q", 0, bar_q)
+            load("k", g + ns, bar_k[g % ns])
+            if g > 0:
+                load("v", g - 1 + ns, bar_v[(g - 1) % ns])
+            if fresh:
+                ok = yield from cta.wait(bar_q, q_phase & 1)
+                if not ok:
+                    break
+                q_phase += 1
+                cta.pipe.append(bar_s.arrive)
+            g += 1
+        if not ok:
+            cta.pipe.append(bar_end.arrive)
+            yield from cta.drain(bar_end, 0, hasty)
+            for parity in (0, 1):
+                for b in [bar_q] + bar_k + bar_v:
+                    yield from cta.drain(b, parity, hasty)
+
+    def softmax():
+        g = tile = 0
+        ok = True
+        for n in blocks:
+            for _ in range(n):
+                ok = yield from cta.wait(bar_s, g & 1)
+                if not ok:
+                    break
+                bar_p.arrive()
+                g += 1
+            if ok and n:
+                ok = yield from cta.wait(bar_o, tile & 1)
+                tile += ok
+            if not ok:
+                break
+        if not ok and not leaves:
+            yield from cta.drain(bar_o, tile & 1, hasty)
+
+    cta.run([issuer()] + [softmax() for _ in range(warps)])
+
+
+@pytest.mark.parametrize("ns", [3, 2])
+@pytest.mark.parametrize("blocks", [[1], [7], [1, 1, 1, 1], [3, 0, 1, 5], [0, 0], [6, 2, 9]])
+def test_tile_kernel_gives_up(ns, blocks):
+    for seed in range(120):
+        tiles(blocks, ns, seed, tired=(0.0, 0.02, 0.2)[seed % 3])
+
+
+@pytest.mark.parametrize("mistake", ["hasty", "leaves"])
+def test_tile_model_shows_mistakes(mistake):
+    n = 0
+    for seed in range(600):
+        try:
+            tiles([2, 3], 3, seed, 0.1, **{mistake: True})
         except (Fault, AssertionError):
             n += 1
     assert n > 0
