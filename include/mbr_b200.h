@@ -303,9 +303,9 @@ MBR_API int mbr_op_attention(const void* d_q, const void* d_k, const void* d_v, 
  * extend split_qkv_heads_rotary and scaled_dot_product_attention.
  * All of these enqueue on `stream` and return without synchronising, allocate
  * no device memory and may be captured into a CUDA graph (call the attention
- * once before the capture: its first call on a device allocates one host-mapped
- * word).  Calls on different streams are independent, each with a workspace
- * (16-byte aligned device memory, contents free) of its own.  The device that is
+ * once before the capture: the first call allocates host-mapped error words,
+ * see mbr_op_stream_check).  Calls on different streams are independent, each
+ * with a workspace (16-byte aligned device memory, contents free) of its own.  The device that is
  * current at the call must own the buffers and the stream.  Tokens, heads or
  * sequences of zero make a call that does nothing. */
 
@@ -383,8 +383,9 @@ MBR_API int mbr_op_cache_read(const mbr_kv_cache* cache, const int32_t* d_pos, c
  * d_gates [seqs][q_tokens][q_heads] fp32 or null.  dim_head a multiple of 8 up
  * to 128.
  * fp16/bf16 run on the tensor cores when pointers and strides are multiples of
- * 16 bytes; other layouts and fp32 on the CUDA cores.  The first call after a
- * kernel-side wait ran out returns MBR_ERR_TIMEOUT. */
+ * 16 bytes; other layouts and fp32 on the CUDA cores.  Returns what
+ * mbr_op_stream_check would return, and launches nothing, if an earlier
+ * attention call on this stream ran out of a kernel-side wait. */
 MBR_API int mbr_op_window_attention(const mbr_view* q, const mbr_view* k, const mbr_view* v, const mbr_view* out,
                                     int64_t seqs, int64_t q_tokens, int64_t kv_tokens, int q_heads, int kv_heads,
                                     int dim_head, const int32_t* d_q_len, const int32_t* d_kv_len, int left,
@@ -409,6 +410,19 @@ MBR_API int mbr_op_cache_attention(const mbr_view* q, const mbr_kv_cache* cache,
 /* Bytes of workspace such a call needs (0: none); host arithmetic only. */
 MBR_API int mbr_op_cache_attention_workspace(const mbr_kv_cache* cache, int64_t tokens, int q_heads, int left,
                                              int right, int64_t* bytes);
+
+/* Every wait inside the attention kernels is bounded.  One that runs out sets
+ * the error word of the stream that the call was made (or captured) on; what
+ * that call and the attention calls behind it wrote is void until the word is
+ * cleared.  mbr_op_stream_check waits for the stream, clears its word and
+ * returns MBR_ERR_TIMEOUT if it was set (MBR_ERR_CUDA: a kernel found its shared
+ * memory misaligned).  Call it after the last call of a sequence, and after
+ * graph replays, which neither look at the word nor clear it: with the stream
+ * that was captured, once the replays have run.  mbr_op_stream_error_word gives
+ * the word's address (host memory, 0: none, valid as long as the process), for
+ * a look without waiting.  Words are kept by device and stream handle. */
+MBR_API int mbr_op_stream_check(void* stream);
+MBR_API int mbr_op_stream_error_word(void* stream, volatile int** word);
 
 /* Host tables of MelBandRoformer::compute_rotary_cos_sin
  * (src/model_mel_band_roformer.cu:270-300): h_cos, h_sin [L][dim_head/2]. */

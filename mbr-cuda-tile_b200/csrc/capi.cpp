@@ -662,6 +662,17 @@ MBR_API int mbr_op_cache_attention_workspace(const mbr_kv_cache* cache, int64_t 
     });
 }
 
+MBR_API int mbr_op_stream_check(void* stream) {
+    return guard([&] { mbr::streamops::stream_check((cudaStream_t)stream); });
+}
+
+MBR_API int mbr_op_stream_error_word(void* stream, volatile int** word) {
+    return guard([&] {
+        need(word, "null argument");
+        *word = mbr::streamops::stream_error_word((cudaStream_t)stream);
+    });
+}
+
 MBR_API int mbr_rope_tables(int L, int dim_head, float* h_cos, float* h_sin) {
     return guard([&] {
         need(h_cos && h_sin && L > 0 && dim_head > 0 && dim_head % 2 == 0, "bad argument");

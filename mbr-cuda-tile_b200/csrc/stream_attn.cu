@@ -18,21 +18,6 @@ int stream_device() {
     return dev;
 }
 
-int* stream_error_word() {
-    // one word for all devices, visible to each (portable); never freed
-    static int* const host = [] {
-        int* p = nullptr;
-        MBR_CUDA(cudaHostAlloc((void**)&p, sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable));
-        *p = 0;
-        return p;
-    }();
-    if (__atomic_load_n(host, __ATOMIC_RELAXED) != 0) {
-        __atomic_store_n(host, 0, __ATOMIC_RELAXED);
-        throw Error(ERR_TIMEOUT, "an earlier streaming attention call ran out of a kernel-side wait");
-    }
-    return host;  // unified addressing: the device uses the same address
-}
-
 namespace {
 
 // Attention over an fp32 cache, a CTA a row: LANES lanes (four channels each) hold a
@@ -219,9 +204,11 @@ void window_attention(const mbr_view& q, const mbr_view& k, const mbr_view& v, c
     if (few_rows(a) && step_supported(a, dtype, false)) {
         const StepPlan pl = plan_of(a, false, Nk);
         MBR_CHECK(pl.bytes == 0 || (workspace && workspace_bytes >= pl.bytes), "window_attention: workspace too small");
+        raise_stream_error(st);
         attend_step(a, dtype, false, false, pl, workspace, st);
         return;
     }
+    raise_stream_error(st);
     if (tile_supported(a, dtype)) {
         attend_tiles(a, dtype, st);
         return;
@@ -250,9 +237,11 @@ void cache_attention(const mbr_view& q, const mbr_kv_cache& c, const mbr_view& o
     if (step_supported(a, c.dtype, true)) {
         const StepPlan pl = plan_of(a, q4, a.slots);
         MBR_CHECK(pl.bytes == 0 || (workspace && workspace_bytes >= pl.bytes), "cache_attention: workspace too small");
+        raise_stream_error(st);
         attend_step(a, c.dtype, true, q4, pl, workspace, st);
         return;
     }
+    raise_stream_error(st);
     launch_rows(a, st);
 }
 

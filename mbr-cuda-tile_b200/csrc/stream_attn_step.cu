@@ -841,7 +841,7 @@ void attend_step(const AttnArgs& a, int dtype, bool cached, bool q4, const StepP
         p.k_tok = a.k_tok * es, p.k_head = a.k_head * es, p.k_seq = a.k_seq * es;
         p.v_tok = a.v_tok * es, p.v_head = a.v_head * es, p.v_seq = a.v_seq * es;
     }
-    p.err = stream_error_word();
+    p.err = stream_error_word(st);
     if (dtype == DT_BF16) {
         if (!cached) dispatch<__nv_bfloat16, false, false>(p, st);
         else if (q4) dispatch<__nv_bfloat16, true, true>(p, st);

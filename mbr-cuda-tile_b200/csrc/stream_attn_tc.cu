@@ -638,7 +638,7 @@ void attend_tiles(const AttnArgs& a, int dtype, cudaStream_t st) {
     p.by_groups = FastDiv((unsigned)p.groups);
     p.by_pack = FastDiv((unsigned)p.pack);
     p.scale_log2 = a.scale * 1.4426950408889634f;
-    p.err = stream_error_word();
+    p.err = stream_error_word(st);
     CUtensorMap q, k, v;
     make_map(&q, a.q, a.q_seq, a.q_tok, a.q_head, a.D, a.Hq, a.Nq, a.seqs, p.pack, p.tokens, dtype);
     make_map(&k, a.k, a.k_seq, a.k_tok, a.k_head, a.D, a.Hkv, a.Nk, a.seqs, 1, KB, dtype);

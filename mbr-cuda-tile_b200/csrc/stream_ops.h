@@ -37,10 +37,13 @@ int64_t cache_attention_workspace(const mbr_kv_cache& c, int64_t tokens, int Hq,
 // Current device (checked against the per-device tables below).
 constexpr int kMaxStreamDevices = 64;
 int stream_device();
-// Error word that the attention kernels' bounded waits set: host memory that
-// the device writes, so the host sees it without a copy.  Throws if it is set
-// (and clears it): the call before ran out of a wait.
-int* stream_error_word();
+// Error word that the bounded waits of this stream's attention kernels set
+// (KERR_* of sm100.cuh), host-mapped, never freed.
+int* stream_error_word(cudaStream_t st);
+// Throws if the stream's word is set, and clears it: an earlier call ran out of a wait.
+void raise_stream_error(cudaStream_t st);
+// The same after what the stream holds has run.
+void stream_check(cudaStream_t st);
 
 // Checks a cache's sizes and type; check_cache its buffers too (true when its rows are 4-bit codes).
 void check_cache_fields(const mbr_kv_cache& c);

@@ -32,6 +32,7 @@ EXPORTS = [
     "mbr_op_rms_norm", "mbr_op_add", "mbr_op_gelu", "mbr_op_sigmoid_gate", "mbr_op_rope", "mbr_op_attention", "mbr_op_linear", "mbr_op_ffn",
     "mbr_op_qk_norm_rope", "mbr_op_cache_append", "mbr_op_cache_read", "mbr_op_window_attention",
     "mbr_op_cache_attention", "mbr_op_window_attention_workspace", "mbr_op_cache_attention_workspace",
+    "mbr_op_stream_check", "mbr_op_stream_error_word",
     "mbr_rope_tables",
     "mbr_op_band_gather", "mbr_op_mask_scatter", "mbr_op_stft", "mbr_op_istft", "mbr_op_istft_noalloc",
     "mbr_plan_shard", "mbr_wav_info", "mbr_wav_read", "mbr_wav_write",
@@ -103,6 +104,8 @@ def lib():
         L.mbr_op_cache_attention.argtypes = [vp, vp, vp, vp, i64, c_int, c_int, c_int, c_float, fp, vp, i64, vp]
         L.mbr_op_window_attention_workspace.argtypes = [i64, i64, i64] + [c_int] * 7 + [i64p]
         L.mbr_op_cache_attention_workspace.argtypes = [vp, i64, c_int, c_int, c_int, i64p]
+        L.mbr_op_stream_check.argtypes = [vp]
+        L.mbr_op_stream_error_word.argtypes = [vp, vp]
         L.mbr_rope_tables.argtypes = [c_int, c_int, fp, fp]
         L.mbr_op_band_gather.argtypes = [vp, fp, c_int, c_int, fp, c_int, vp]
         L.mbr_op_mask_scatter.argtypes = [vp, fp, fp, c_int, c_int, c_int, fp, c_int, vp]
@@ -364,6 +367,12 @@ def op_cache_attention(q, cache, length, left=-1, right=0, scale=0.0, gates=None
     """The attention of op_window_attention for the newest tokens over a cache that holds them: q [seqs, tokens,
     q_heads, dim_head], length int32 [seqs] tokens appended so far (these included); the cache's sinks stay visible."""
     return (_CALLS or _calls()).cache_attention(q, cache, length, left, right, scale, gates, out, stream)
+
+
+def op_stream_check(stream=None):
+    """Waits for the stream and raises MBRError if a kernel-side wait of an attention call above ran out on it: to be
+    called after the last one, and after graph replays (with the stream that was captured)."""
+    _check(lib().mbr_op_stream_check(_stream(stream)))
 
 
 def op_stft(sig, hop=441, stream=None):
