@@ -285,15 +285,24 @@ def _elsewhere(dev, name, args):
         return getattr(_CALLS, name)(*args)
 
 
+def _torch_stream(stream, device):
+    """torch's object of a stream given as such or as a handle."""
+    import torch
+
+    if isinstance(stream, torch.cuda.Stream):
+        return stream
+    handle = stream if isinstance(stream, int) else stream.cuda_stream
+    # 0 and 1 both name the default stream; ExternalStream(0) would be a new one
+    return torch.cuda.default_stream(device) if handle in (0, 1) else torch.cuda.ExternalStream(handle, device=device)
+
+
 def _workspace(n, device, stream):
     """n bytes of device memory for one call on `stream` (None: the current one); freed in that stream's order."""
     import torch
 
     if stream is None:
         return torch.empty(n, dtype=torch.uint8, device=device)
-    if isinstance(stream, int):
-        stream = torch.cuda.ExternalStream(stream, device=device)
-    with torch.cuda.stream(stream):
+    with torch.cuda.stream(_torch_stream(stream, device)):
         return torch.empty(n, dtype=torch.uint8, device=device)
 
 
