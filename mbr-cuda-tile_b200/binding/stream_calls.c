@@ -31,7 +31,7 @@ static PyObject *t_f32, *t_i32, *t_u8;    /* torch dtypes */
 static PyObject* t_codes;                 /* {dtype: code} */
 static PyObject *p_empty_like, *p_kwargs; /* torch.empty_like and {"memory_format": torch.contiguous_format} */
 static PyObject *p_stream, *p_device;     /* current stream's handle of a device; current device */
-static PyObject *p_check, *p_elsewhere, *p_workspace;
+static PyObject *p_check, *p_elsewhere, *p_workspace, *p_like_on;
 static PyObject *s_stride, *s_shape, *s_dtype, *s_get_device, *s_data_ptr, *s_contiguous, *s_device, *s_desc, *s_dev,
     *s_new, *s_cuda_stream;
 
@@ -148,9 +148,11 @@ static int device_of(PyObject* t, long long* dev) {
     return *dev >= 0 ? 0 : refuse("tensors must be on a CUDA device");
 }
 
-static PyObject* like(PyObject* t) { /* new contiguous tensor of the same shape and type */
-    PyObject* args[1] = {t};
-    return PyObject_VectorcallDict(p_empty_like, args, 1, p_kwargs);
+/* New contiguous tensor of the same shape and type, the memory of `stream` (None: the current one). */
+static PyObject* like(PyObject* t, PyObject* stream) {
+    PyObject* args[2] = {t, stream};
+    return stream == Py_None ? PyObject_VectorcallDict(p_empty_like, args, 1, p_kwargs)
+                             : PyObject_Vectorcall(p_like_on, args, 2, NULL);
 }
 
 /* 1: `dev` is current and *handle is the stream to use; 0: another device is current; -1: error. */
@@ -295,8 +297,8 @@ static PyObject* call_norm(PyObject* self, PyObject* const* a, Py_ssize_t n) {
         if (on == 0) res = elsewhere(dev, "qk_norm_rope", a, n);
         goto done;
     }
-    qo = a[9] == Py_None ? like(q) : Py_NewRef(a[9]);
-    ko = a[10] == Py_None ? like(k) : Py_NewRef(a[10]);
+    qo = a[9] == Py_None ? like(q, a[11]) : Py_NewRef(a[9]);
+    ko = a[10] == Py_None ? like(k, a[11]) : Py_NewRef(a[10]);
     if (!qo || !ko || rows("q_out", qo, dt, dev, &rqo) || rows("k_out", ko, dt, dev, &rko)) goto done;
     for (int i = 0; i < 4; ++i)
         if (rqo.n[i] != rq.n[i] || rko.n[i] != rk.n[i]) {
@@ -380,8 +382,8 @@ static PyObject* call_read(PyObject* self, PyObject* const* a, Py_ssize_t n) {
         shape = Py_BuildValue("(LLii)", (long long)seqs, tokens, x.c->kv_heads, x.c->dim_head);
         if (!shape) goto done;
     }
-    ko = a[4] == Py_None ? PyObject_CallMethodOneArg(a[0], s_new, shape) : Py_NewRef(a[4]);
-    vo = a[5] == Py_None && ko ? PyObject_CallMethodOneArg(a[0], s_new, shape) : Py_NewRef(a[5]);
+    ko = a[4] == Py_None ? PyObject_CallMethodObjArgs(a[0], s_new, shape, a[6], NULL) : Py_NewRef(a[4]);
+    vo = a[5] == Py_None && ko ? PyObject_CallMethodObjArgs(a[0], s_new, shape, a[6], NULL) : Py_NewRef(a[5]);
     if (!ko || !vo || rows("k", ko, x.dtype, x.dev, &k) || rows("v", vo, x.dtype, x.dev, &v)) goto done;
     if (!same_rows(&k, x.c) || !same_rows(&v, x.c) || k.n[1] != tokens || v.n[1] != tokens) {
         refuse("k and v must be [seqs, tokens, kv_heads, dim_head] of the cache");
@@ -432,7 +434,7 @@ static PyObject* call_window(PyObject* self, PyObject* const* a, Py_ssize_t n) {
         if (on == 0) res = elsewhere(dev, "window_attention", a, n);
         goto done;
     }
-    out = a[10] == Py_None ? like(a[0]) : Py_NewRef(a[10]);
+    out = a[10] == Py_None ? like(a[0], a[11]) : Py_NewRef(a[10]);
     if (!out || rows("out", out, dt, dev, &o)) goto done;
     for (int i = 0; i < 4; ++i)
         if (o.n[i] != q.n[i]) {
@@ -480,7 +482,7 @@ static PyObject* call_cache(PyObject* self, PyObject* const* a, Py_ssize_t n) {
         if (on == 0) res = elsewhere(x.dev, "cache_attention", a, n);
         goto done;
     }
-    out = a[7] == Py_None ? like(a[0]) : Py_NewRef(a[7]);
+    out = a[7] == Py_None ? like(a[0], a[8]) : Py_NewRef(a[7]);
     if (!out || rows("out", out, x.dtype, x.dev, &o)) goto done;
     for (int i = 0; i < 4; ++i)
         if (o.n[i] != q.n[i]) {
@@ -559,15 +561,15 @@ done:
 static PyObject* call_bind(PyObject* self, PyObject* args) {
     unsigned long long f[7];
     PyObject* o[12];
-    if (!PyArg_ParseTuple(args, "(KKKKKKK)(OOOOOOOOOOO)", &f[0], &f[1], &f[2], &f[3], &f[4], &f[5], &f[6], &o[0], &o[1],
-                          &o[2], &o[3], &o[4], &o[5], &o[6], &o[7], &o[8], &o[9], &o[10]))
+    if (!PyArg_ParseTuple(args, "(KKKKKKK)(OOOOOOOOOOOO)", &f[0], &f[1], &f[2], &f[3], &f[4], &f[5], &f[6], &o[0], &o[1],
+                          &o[2], &o[3], &o[4], &o[5], &o[6], &o[7], &o[8], &o[9], &o[10], &o[11]))
         return NULL;
     *(void**)&f_norm = (void*)f[0], *(void**)&f_append = (void*)f[1], *(void**)&f_read = (void*)f[2];
     *(void**)&f_window = (void*)f[3], *(void**)&f_window_ws = (void*)f[4], *(void**)&f_cache = (void*)f[5];
     *(void**)&f_cache_ws = (void*)f[6];
-    PyObject** to[11] = {&t_f32,    &t_i32,    &t_u8,    &t_codes,     &p_empty_like, &p_kwargs,
-                         &p_stream, &p_device, &p_check, &p_elsewhere, &p_workspace};
-    for (int i = 0; i < 11; ++i) Py_XSETREF(*to[i], Py_NewRef(o[i]));
+    PyObject** to[12] = {&t_f32,    &t_i32,    &t_u8,    &t_codes,     &p_empty_like, &p_kwargs,
+                         &p_stream, &p_device, &p_check, &p_elsewhere, &p_workspace,  &p_like_on};
+    for (int i = 0; i < 12; ++i) Py_XSETREF(*to[i], Py_NewRef(o[i]));
     Py_RETURN_NONE;
 }
 

@@ -244,6 +244,8 @@ def op_attention(q, k, v, scale=0.0, gates=None, out=None, stream=None):
 
 
 # ---- streaming time-axis attention ----
+# Each call runs on `stream` (None: the current one; a torch stream or a handle).  Outputs that a call allocates are that
+# stream's memory, as if it had been the current one: other streams wait for it before they read them.
 _CALLS = None  # the extension that makes these calls, see _calls()
 
 
@@ -272,7 +274,8 @@ def _calls():
         module.bind(
             tuple(ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in names),
             (torch.float32, torch.int32, torch.uint8, {torch.float32: FP32, torch.float16: FP16, torch.bfloat16: BF16},
-             torch.empty_like, {"memory_format": torch.contiguous_format}, stream, device, _check, _elsewhere, _workspace))
+             torch.empty_like, {"memory_format": torch.contiguous_format}, stream, device, _check, _elsewhere, _workspace,
+             _like_on))
         _CALLS = module
     return _CALLS
 
@@ -306,6 +309,23 @@ def _workspace(n, device, stream):
         return torch.empty(n, dtype=torch.uint8, device=device)
 
 
+def _empty_on(stream, shape, dtype, device):
+    """An uninitialised output of a call on `stream` (None: the current one): that stream's memory, which the current
+    stream, whose work may read it, has to be done with before it is used again."""
+    import torch
+
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(_torch_stream(stream, device)):
+        t = torch.empty(shape, dtype=dtype, device=device)
+    t.record_stream(torch.cuda.current_stream(device))
+    return t
+
+
+def _like_on(t, stream):
+    return _empty_on(stream, t.shape, t.dtype, t.device)
+
+
 def op_qk_norm_rope(q, k, gamma_q=None, gamma_k=None, cos=None, sin=None, pos=None, pairs=(), eps=1e-6, q_out=None,
                     k_out=None, stream=None):
     """q [seqs, tokens, q_heads, dim_head], k [seqs, tokens, kv_heads, dim_head] -> both normed over each head
@@ -330,9 +350,9 @@ class KVCache:
          self.bits) = (_CALLS or _calls()).cache_fields(k, v, k_scale, v_scale, sinks)
         self.k, self.v, self.k_scale, self.v_scale, self.sinks = k, v, k_scale, v_scale, sinks
 
-    def new(self, shape):
-        """An uninitialised tensor of the cache's type on its device."""
-        return (self.k_scale if self.bits else self.k).new_empty(shape)
+    def new(self, shape, stream=None):
+        """An uninitialised tensor of the cache's type on its device, the memory of `stream` (None: the current one)."""
+        return _empty_on(stream, shape, self.dtype, self.k.device)
 
     @classmethod
     def empty(cls, seqs, kv_heads, slots, dim_head, dtype, sinks=0, bits=0, device="cuda"):

@@ -68,3 +68,30 @@ def test_the_split_call_needs_a_workspace(torch_cuda):
     n = ctypes.c_int64()
     assert cudasep.lib().mbr_op_cache_attention_workspace(cache.desc, 1, 2, -1, 0, ctypes.byref(n)) == 0
     assert n.value > 0
+
+
+def test_outputs_belong_to_the_stream_of_their_call(torch_cuda):
+    torch = torch_cuda
+    import cudasep
+
+    q = torch.randn((2, 5, 2, 64), device="cuda").half()
+    cache = cudasep.KVCache.empty(2, 2, 16, 64, torch.float16)
+    pos = torch.zeros(2, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    calls = [lambda s: cudasep.op_qk_norm_rope(q, q, stream=s),
+             lambda s: (cudasep.op_window_attention(q, q, q, stream=s),),
+             lambda s: cudasep.op_cache_append(cache, q, q, pos, stream=s) or cudasep.op_cache_read(cache, pos, 5, stream=s),
+             lambda s: (cudasep.op_cache_attention(q, cache, pos + 5, stream=s),)]
+    for call in calls:
+        want = call(None)
+        torch.cuda.synchronize()
+        for stream, handle in _ways(torch):
+            other = torch.cuda.Stream()
+            with torch.cuda.stream(other):
+                got = call(stream)
+            torch.cuda.synchronize()
+            assert [_owner(torch, t) for t in got] == [handle] * len(got)
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+            with torch.cuda.stream(other):
+                assert all(_owner(torch, t) == other.cuda_stream for t in call(None))
+            torch.cuda.synchronize()
