@@ -33,7 +33,7 @@ static PyObject *p_empty_like, *p_kwargs; /* torch.empty_like and {"memory_forma
 static PyObject *p_stream, *p_device;     /* current stream's handle of a device; current device */
 static PyObject *p_check, *p_elsewhere, *p_workspace, *p_like_on;
 static PyObject *s_stride, *s_shape, *s_dtype, *s_get_device, *s_data_ptr, *s_contiguous, *s_device, *s_desc, *s_dev,
-    *s_new, *s_cuda_stream;
+    *s_new, *s_cuda_stream, *s_cache_dtype;
 
 /* ---- looking at tensors ---- */
 typedef struct {
@@ -235,7 +235,7 @@ typedef struct {
 static int cache_arg(PyObject* o, cache_t* x) {
     x->desc = PyObject_GetAttr(o, s_desc);
     if (!x->desc) return -1;
-    PyObject* d = PyObject_GetAttr(o, s_dtype);
+    PyObject* d = PyObject_GetAttr(o, s_cache_dtype);
     if (!d || !PyBytes_Check(x->desc) || PyBytes_GET_SIZE(x->desc) != sizeof(mbr_kv_cache) || attr_long(o, s_dev, &x->dev)) {
         Py_XDECREF(d), Py_DECREF(x->desc);
         if (!PyErr_Occurred()) refuse("expected a KVCache");
@@ -591,8 +591,9 @@ PyMODINIT_FUNC PyInit__stream_calls(void) {
         const char* text;
     } names[] = {{&s_stride, "stride"},         {&s_shape, "shape"},       {&s_dtype, "dtype"},
                  {&s_get_device, "get_device"}, {&s_data_ptr, "data_ptr"}, {&s_contiguous, "is_contiguous"},
-                 {&s_device, "device"},         {&s_desc, "desc"},         {&s_dev, "dev"},
-                 {&s_new, "new"},               {&s_cuda_stream, "cuda_stream"}};
+                 {&s_device, "device"},         {&s_desc, "_desc"},        {&s_dev, "_dev"},
+                 {&s_new, "new"},               {&s_cuda_stream, "cuda_stream"},
+                 {&s_cache_dtype, "_dtype"}};
     for (size_t i = 0; i < sizeof names / sizeof *names; ++i)
         if (!(*names[i].to = PyUnicode_InternFromString(names[i].text))) return NULL;
     return PyModule_Create(&module);

@@ -9,6 +9,7 @@ shared library is missing or a call fails, an exception is raised.
 from __future__ import annotations
 
 import ctypes
+import operator
 import os
 
 import numpy as np
@@ -340,15 +341,22 @@ class KVCache:
 
     k, v [seqs, kv_heads, slots, dim_head], or uint8 [seqs, kv_heads, slots, dim_head / 2] of 4-bit codes with k_scale,
     v_scale [seqs, kv_heads, slots, dim_head / 32, 2] (step and offset of each 32 channels).  The first `sinks`
-    positions keep their slots, the other slots are a ring."""
+    positions keep their slots, the other slots are a ring.
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "sinks", "ring", "dtype", "dev", "seqs", "kv_heads", "dim_head", "bits",
-                 "desc")
+    The calls use the tensors' addresses, which are taken here: the attributes cannot be set (to restore a stream's state,
+    copy into cache.k, ... or make another KVCache), and copies and pickles are made anew from the tensors."""
+
+    _FIELDS = ("k", "v", "k_scale", "v_scale", "sinks", "ring", "dtype", "dev", "seqs", "kv_heads", "dim_head", "bits",
+               "desc")
+    __slots__ = tuple("_" + n for n in _FIELDS)
 
     def __init__(self, k, v, k_scale=None, v_scale=None, sinks=0):
-        (self.desc, self.dtype, self.dev, self.seqs, self.kv_heads, self.dim_head, self.ring,
-         self.bits) = (_CALLS or _calls()).cache_fields(k, v, k_scale, v_scale, sinks)
-        self.k, self.v, self.k_scale, self.v_scale, self.sinks = k, v, k_scale, v_scale, sinks
+        (self._desc, self._dtype, self._dev, self._seqs, self._kv_heads, self._dim_head, self._ring,
+         self._bits) = (_CALLS or _calls()).cache_fields(k, v, k_scale, v_scale, sinks)
+        self._k, self._v, self._k_scale, self._v_scale, self._sinks = k, v, k_scale, v_scale, sinks
+
+    def __reduce__(self):
+        return KVCache, (self.k, self.v, self.k_scale, self.v_scale, self.sinks)
 
     def new(self, shape, stream=None):
         """An uninitialised tensor of the cache's type on its device, the memory of `stream` (None: the current one)."""
@@ -369,6 +377,10 @@ class KVCache:
         ks, vs = (torch.zeros((seqs, kv_heads, slots, dim_head // 32, 2), dtype=dtype, device=device)
                   for _ in range(2))
         return cls(k, v, ks, vs, sinks=sinks)
+
+
+for _n in KVCache._FIELDS:
+    setattr(KVCache, _n, property(operator.attrgetter("_" + _n)))
 
 
 def op_cache_append(cache, k, v, pos, count=None, stream=None):
