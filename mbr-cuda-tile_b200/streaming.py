@@ -23,7 +23,9 @@ class StreamingTimeAttention:
 
     w_qkv [3 * heads * dim_head, dim], w_gate [heads, dim], w_out [dim, heads * dim_head], gamma_q / gamma_k [dim_head]
     fp32; the matrices in fp16 or bf16, on one GPU.  A frame sees itself, `left` frames before it and the first `sinks`
-    frames of the stream; `bits` 0 keeps the cache in the matrices' type, 4 in 4 bits."""
+    frames of the stream; `bits` 0 keeps the cache in the matrices' type, 4 in 4 bits.  A stream has up to `max_frames`
+    frames (the angle tables are made for as many; 65536 are 10 min 55 s): `prompt` and `step` refuse more and leave the
+    stream as it is."""
 
     def __init__(self, w_qkv, w_gate, w_out, gamma_q, gamma_k, bands, heads, left, sinks=4, bits=0, max_frames=1 << 16):
         import torch
@@ -35,6 +37,7 @@ class StreamingTimeAttention:
         # the first half of each head's pairs turns with the frame, the second with the band
         half = self.dim_head // 2
         self.pairs = [half - half // 2, half // 2]
+        self.max_frames = max_frames
         c, s = cudasep.rope_tables(max(max_frames, bands), self.dim_head)
         self.cos, self.sin = (torch.from_numpy(t).to(self.device) for t in (c, s))
         self.band = torch.arange(bands, dtype=torch.int32, device=self.device)
@@ -49,6 +52,8 @@ class StreamingTimeAttention:
         import torch
 
         n, nb, dim = x.shape
+        if self.frames + n > self.max_frames:  # positions past the tables would be NaN, in the cache too
+            raise ValueError(f"a stream takes up to max_frames = {self.max_frames} frames, got {self.frames} + {n}")
         H, D = self.heads, self.dim_head
         flat = x.reshape(n * nb, dim)
         qkv = cudasep.op_linear(flat, self.w_qkv).view(n, nb, 3 * H, D).transpose(0, 1)
@@ -107,7 +112,8 @@ class StreamingTimeAttention:
         return self._finish(self.attend_step(x), x)
 
 
-def random_layer(bands, dim, heads, dim_head=64, left=100, sinks=4, bits=0, dtype="bf16", seed=0, device="cuda"):
+def random_layer(bands, dim, heads, dim_head=64, left=100, sinks=4, bits=0, dtype="bf16", seed=0, device="cuda",
+                 max_frames=1 << 16):
     """A layer with seeded random weights."""
     import torch
 
@@ -120,7 +126,8 @@ def random_layer(bands, dim, heads, dim_head=64, left=100, sinks=4, bits=0, dtyp
     inner = heads * dim_head
     return StreamingTimeAttention(w(3 * inner, dim, scale=dim ** -0.5).to(dt), w(heads, dim, scale=dim ** -0.5).to(dt),
                                   w(dim, inner, scale=inner ** -0.5).to(dt), 1 + w(dim_head, scale=0.1),
-                                  1 + w(dim_head, scale=0.1), bands, heads, left, sinks, bits)
+                                  1 + w(dim_head, scale=0.1), bands, heads, left, sinks, bits,
+                                  max_frames)
 
 
 def main(argv=None):
@@ -138,7 +145,8 @@ def main(argv=None):
     a = ap.parse_args(argv)
     n = max(2, int(round(100 * a.seconds)))
     x = torch.randn((n, a.bands, a.dim), generator=torch.Generator().manual_seed(1)).cuda()
-    make = dict(bands=a.bands, dim=a.dim, heads=a.heads, left=a.left, sinks=a.sinks, bits=a.bits, dtype=a.dtype)
+    make = dict(bands=a.bands, dim=a.dim, heads=a.heads, left=a.left, sinks=a.sinks, bits=a.bits, dtype=a.dtype,
+                max_frames=n)
     whole = random_layer(**make)
     x = x.to(whole.dtype)
     want = whole.prompt(x)
