@@ -41,6 +41,14 @@ bool check_cache(const mbr_kv_cache& c) {
 
 namespace {
 
+// What x - m and the step are multiplied by before the one goes by the other's
+// reciprocal: a power of two for a bf16 step below fp32's normal range, whose
+// reciprocal would be infinite (2^-133 is the least).
+template <typename T>
+__device__ __forceinline__ float step_scale(float step) {
+    return std::is_same_v<T, __nv_bfloat16> && step < 0x1p-126f ? 0x1p24f : 1.f;
+}
+
 struct RowArgs {
     mbr_kv_cache c;
     mbr_view k, v;
@@ -114,8 +122,9 @@ __global__ void __launch_bounds__(256) cache_rows_kernel(const RowArgs a) {
                         const T sT = from_f32<T>(__fmul_rn(hi - lo, 1.f / 15.f));
                         const float s = to_f32<T>(sT);
                         const T mT = from_f32<T>(__fadd_rn(lo, 8.f * s));
-                        const float m = to_f32<T>(mT), inv = s > 0.f ? __frcp_rn(s) : 0.f;
-                        const float q = rintf(__fmul_rn(__fadd_rn(v, -m), inv)) + 8.f;
+                        const float up = step_scale<T>(s);
+                        const float m = to_f32<T>(mT), inv = s > 0.f ? __frcp_rn(s * up) : 0.f;
+                        const float q = rintf(__fmul_rn(__fadd_rn(v, -m) * up, inv)) + 8.f;
                         int code = (int)fminf(fmaxf(q, 0.f), 15.f);
                         const int other = __shfl_down_sync(0xffffffffu, code, 1);
                         if ((lane & 1) == 0) row[d >> 1] = (uint8_t)(code | (other << 4));
@@ -238,7 +247,8 @@ __global__ void __launch_bounds__(256) cache_vec_kernel(const RowArgs a, int lan
                 const T sT = from_f32<T>(__fmul_rn(hi - lo, 1.f / 15.f));
                 const float st = to_f32<T>(sT);
                 const T mT = from_f32<T>(__fadd_rn(lo, 8.f * st));
-                const float m = to_f32<T>(mT), inv = st > 0.f ? __frcp_rn(st) : 0.f;
+                const float up = step_scale<T>(st);
+                const float m = to_f32<T>(mT), inv = st > 0.f ? __frcp_rn(st * up) : 0.f;
                 // rint((v - m) / st) + 8 within 0..15: adding 1.5 2^23 rounds to an integer; four codes are put
                 // together as one (their sum is below 2^16) in floating point
                 float part[2];
@@ -248,7 +258,8 @@ __global__ void __launch_bounds__(256) cache_vec_kernel(const RowArgs a, int lan
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
                         const T* e = reinterpret_cast<const T*>(w + 2 * half + c);
-                        const float2 d = __fadd2_rn(make_float2(to_f32<T>(e[0]), to_f32<T>(e[1])), make_float2(-m, -m));
+                        const float2 d = __ffma2_rn(make_float2(to_f32<T>(e[0]), to_f32<T>(e[1])), make_float2(up, up),
+                                                    make_float2(-m * up, -m * up));
                         float2 x = __fmul2_rn(d, make_float2(inv, inv));
                         x.x = fminf(fmaxf(x.x, -8.f), 7.f), x.y = fminf(fmaxf(x.y, -8.f), 7.f);
                         x = __fadd2_rn(x, make_float2(12582920.f, 12582920.f));
