@@ -68,7 +68,7 @@ __device__ __forceinline__ float kv_elem(const AttnArgs& a, bool val, int64_t s,
         } else {
             const int byte = ((const uint8_t*)(val ? a.v : a.k))[row * (a.D / 2) + (d >> 1)];
             const T* sm = (const T*)(val ? a.v_scale : a.k_scale) + (row * (a.D / kGroup) + d / kGroup) * 2;
-            return to_f32<T>(code_value<T>((byte >> ((d & 1) * 4)) & 15, to_f32<T>(sm[0]), to_f32<T>(sm[1])));
+            return to_f32<T>(code_value<T>((byte >> ((d & 1) * 4)) & 15, sm[0], sm[1]));
         }
     }
 }

@@ -31,12 +31,11 @@ __device__ __forceinline__ int64_t slot_of(int p, int sinks, int ring) {
     return p < sinks ? p : sinks + (int64_t)((unsigned)(p - sinks) % (unsigned)ring);
 }
 
-// The value that code c of a group with step s and offset m stands for: exact
-// in fp32 (a 4-bit integer times a 16-bit value) up to the sum's rounding,
-// then rounded to the cache's type.
+// The value that code c of a group with step s and offset m stands for, m + s (c
+// - 8): one rounding, to the cache's type (an fp32 sum would be a second one).
 template <typename T>
-__device__ __forceinline__ T code_value(int c, float s, float m) {
-    return from_f32<T>(m + s * (float)(c - 8));
+__device__ __forceinline__ T code_value(int c, T s, T m) {
+    return __hfma(s, from_f32<T>((float)(c - 8)), m);
 }
 
 // Keys of a query at position p over `len` keys: [lo, hi) and [0, first).

@@ -1,4 +1,5 @@
-"""4-bit caches at the edges of their definition: steps below fp32's normal range."""
+"""4-bit caches at the edges of their definition: steps below fp32's normal range, and values whose exact sum lies next to a
+tie of the cache's type (one rounding, in every place that widens codes)."""
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -43,3 +44,49 @@ def test_steps_below_the_normal_range(torch_cuda, aligned):
     assert torch.equal(cache.k_scale[0, 0, :, :, 1].cpu().double(), mid[0, :, 0, :, 0])
     got = torch.stack([cache.k & 15, cache.k >> 4], -1).flatten(-2)[0, 0].cpu().double()
     assert torch.equal(got[sure], want[sure])
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("aligned", [True, False])
+def test_values_are_rounded_once(torch_cuda, dtype, aligned):
+    """m + s (c - 8) next to a tie of the type, nearer than fp32 can tell: read back and seen by the attention (one key a
+    sequence, so that its value is the output) as the exact sum rounded once."""
+    torch = torch_cuda
+    import cudasep
+
+    dt, bits, tiny = {"fp16": (torch.float16, 10, 2.0 ** -24), "bf16": (torch.bfloat16, 7, 2.0 ** -40)}[dtype]
+    S, D = 4, 64
+    s = torch.tensor([1 + 2.0 ** -bits, 1 + 3 * 2.0 ** -bits, 1 - 2.0 ** (-bits - 1), 1.0], dtype=torch.float64)
+    m = torch.tensor([-tiny, tiny, -tiny, tiny], dtype=torch.float64)
+    codes = torch.arange(D) % 16
+    exact = (s[:, None] * (codes - 8) + m[:, None])  # 64 bits hold every sum
+    fp32 = (s[:, None].float() * (codes - 8).float() + m[:, None].float()).to(dt).double()
+    # one rounding from 64 bits: the two neighbours, the nearer one
+    near = exact.float().to(dt).double()
+    ulp = 2.0 ** (torch.floor(torch.log2(exact.abs().clamp_min(2.0 ** -14))) - bits)
+    cands = torch.stack([near - ulp, near, near + ulp])
+    want = torch.gather(cands, 0, (cands - exact).abs().argmin(0, keepdim=True))[0]
+    assert (want != fp32).any()  # rounding twice shows
+    cache = cudasep.KVCache.empty(S, 1, 1, D, dt, bits=4)
+    cache.k.copy_((codes[0::2] | codes[1::2] << 4).to(torch.uint8).expand(S, 1, 1, D // 2))
+    cache.v.copy_(cache.k)
+    for t in (cache.k_scale, cache.v_scale):
+        t[..., 0], t[..., 1] = s.to(dt).cuda().view(S, 1, 1, 1), m.to(dt).cuda().view(S, 1, 1, 1)
+    assert torch.equal(cache.k_scale[:, 0, 0, 0].double().cpu(), torch.stack([s, m], -1))
+    zero = torch.zeros(S, dtype=torch.int32, device="cuda")
+    buf = torch.zeros((S, 1, 1, D + 8 * aligned + 1 * (not aligned)), dtype=dt, device="cuda")
+    out = buf[..., 8:] if aligned else buf[..., 1:]
+    k, v = cudasep.op_cache_read(cache, zero, 1, k=out, v=torch.empty_like(out))
+    assert torch.equal(k[:, 0, 0].cpu().double(), want) and torch.equal(v[:, 0, 0].cpu().double(), want)
+    q = torch.zeros((S, 1, 1, D), dtype=dt, device="cuda")
+    got = cudasep.op_cache_attention(q, cache, zero + 1)
+    assert torch.equal(got[:, 0, 0].cpu().double(), want)
+    # the form that takes rows that are not finite again, by a NaN in a key: the values of the other keys stay
+    q = torch.ones((S, 1, 1, D), dtype=dt, device="cuda")
+    big = cudasep.KVCache.empty(S, 1, 3, D, dt, bits=4)
+    for a, b in ((big.k, cache.k), (big.v, cache.v), (big.k_scale, cache.k_scale), (big.v_scale, cache.v_scale)):
+        a[:, :, :1] = b
+    big.v_scale[:, :, 1:] = float("nan")
+    two = torch.cat([q, q], 1)
+    got = cudasep.op_cache_attention(two, big, zero + 2)  # row 0 sees key 0 only, row 1 the NaN too
+    assert torch.equal(got[:, 0, 0].cpu().double(), want) and got[:, 1].isnan().all()
