@@ -168,14 +168,22 @@ AttnArgs window_args(const mbr_view& q, const mbr_view& k, const mbr_view& v, co
     return a;
 }
 
-// The form for few queries: it splits the keys of 16 rows at a time, where the tile
-// form takes 128 rows and all their keys.  16 rows (us, few-token form / tiles; heads
-// of 64): 60 sequences of 801 keys and 8 key heads 35 / 33, of 2 key heads 14.5 / 16,
-// 8 sequences of 4001 keys 36 / 57.  32 rows read the keys twice: 58 / 33, 21 / 16, and
-// 37 / 57 where the tiles would leave most SMs idle; 64 rows 114 / 34, 33 / 16, 64 / 57.
+// The form for few queries: it takes 16 rows at a time, a CTA or more each, and splits
+// their keys over its warps; the tile form takes 128 rows and all their keys.
+bool takes_few(const AttnArgs& a) { return (int64_t)a.Nq * a.G <= 16; }
+// Where it is the faster one: up to 16 rows of heads up to 64; otherwise (it reads the keys once for
+// each 16 rows, and has half the keys in flight past heads of 64) up to 32 rows if they make fewer CTAs than
+// there are SMs.  us, few-token form / tiles, for 1, 16 and 32 rows a key head, fp16:
+//   heads of 32, 480 key heads (sequences x heads) of 1301 keys 27/46  31/46  56/47
+//   heads of 64, 480 of 1301 42/49  49/49  84/49;   240 of 1301 26/27  29/26  48/26
+//                 64 of 1301 16/23  18/23  18/23;    24 of 8001 20/109 21/109 30/109
+//                 64 of 300   8/9   10/9   11/9  (it loses where keys are few)
+//   heads of 128, 240 of 1301 47/43 53/43  -;       160 of 4001 122/102 131/102  -
+//                128 of 1301 28/31  33/31 52/28;     64 of 4001 65/94 72/94 72/94
+//                  8 of 1301 27/27  30/27 30/27;     24 of 8001 32/166 39/173 57/174
 bool few_rows(const AttnArgs& a) {
     const int64_t rows = (int64_t)a.Nq * a.G;
-    return rows <= 16 || (rows <= 32 && a.seqs * a.Hkv < 148);
+    return (rows <= 16 && a.D <= 64) || (rows <= 32 && a.seqs * a.Hkv * ceil_div(rows, 16) < 148);
 }
 
 StepPlan plan_of(const AttnArgs& a, bool q4, int64_t held) {
@@ -189,7 +197,7 @@ int64_t window_attention_workspace(int64_t seqs, int64_t Nq, int64_t Nk, int Hq,
     const mbr_view none{};
     const AttnArgs a =
         window_args(none, none, none, none, seqs, Nq, Nk, Hq, Hkv, D, left, right, sinks, 0.f, nullptr, dtype);
-    if (seqs == 0 || Nq == 0 || Hq == 0 || dtype == DT_F32 || !few_rows(a)) return 0;
+    if (seqs == 0 || Nq == 0 || Hq == 0 || dtype == DT_F32 || !(few_rows(a) || takes_few(a))) return 0;
     return plan_of(a, false, Nk).bytes;
 }
 
@@ -201,7 +209,8 @@ void window_attention(const mbr_view& q, const mbr_view& k, const mbr_view& v, c
     if (seqs == 0 || Nq == 0 || Hq == 0) return;
     MBR_CHECK(q.data && out.data && (Nk == 0 || (k.data && v.data)), "window_attention: null buffer");
     a.q_len = q_len, a.kv_len = kv_len;
-    if (few_rows(a) && step_supported(a, dtype, false)) {
+    const bool tiles = tile_supported(a, dtype);
+    if (step_supported(a, dtype, false) && (few_rows(a) || (takes_few(a) && !tiles))) {
         const StepPlan pl = plan_of(a, false, Nk);
         MBR_CHECK(pl.bytes == 0 || (workspace && workspace_bytes >= pl.bytes), "window_attention: workspace too small");
         raise_stream_error(st);
@@ -209,7 +218,7 @@ void window_attention(const mbr_view& q, const mbr_view& k, const mbr_view& v, c
         return;
     }
     raise_stream_error(st);
-    if (tile_supported(a, dtype)) {
+    if (tiles) {
         attend_tiles(a, dtype, st);
         return;
     }

@@ -628,9 +628,11 @@ void attend_tiles(const AttnArgs& a, int dtype, cudaStream_t st) {
     MBR_CHECK(sg * p.qtiles < (1ll << 30), "attention: too many tiles");
     p.ntiles = (unsigned)(sg * p.qtiles);
     // With a limit on the right the earliest queries see fewest keys.  Later ones go first, so that what is left at the
-    // end is small, where there is no limit on the left (all differ) or the tiles make few rounds (4 rounds: 91 us
-    // against 99; 8 rounds: 95 against 94).  Otherwise a sequence-head's tiles go together and find its keys in L2; six
-    // rounds of windows fit there in any order.
+    // end is small, where there is no limit on the left (all differ) or the tiles make few rounds.  Otherwise a
+    // sequence-head's tiles go together and find its keys in L2; six rounds of windows mostly fit there in any order.
+    // us, later first / together, at 2, 4, 6, 8 and 20 rounds: heads of 64, 250 + 20 keys 30/34 53/56 77/78 99/100 248/237;
+    // heads of 128, 4 query heads a key head, 400 + 7 keys 28/29 53/54 76/78 97/99 250/226; heads of 128, 100 keys 27/30
+    // 47/47 74/70 91/83 236/201.
     const bool wide = a.D > 64;
     const unsigned round = 148 * (wide ? TileCfg<2>::CTAS : TileCfg<1>::CTAS);
     p.last_first = a.right >= 0 && (a.left < 0 || p.ntiles <= 6 * round);

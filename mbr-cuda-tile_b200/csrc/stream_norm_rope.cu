@@ -231,8 +231,10 @@ void launch_steps(NormRopeArgs a, cudaStream_t st) {
 // With few tokens a step is one head a lane group (more warps share the latency),
 // otherwise four (more loads in flight a warp).  16 heads of 64 in fp16 (us, one /
 // four): 480 tokens 2.6 / 3.3, 960 tokens 3.0 / 3.4, 3840 tokens 5.8 / 5.4, 48060
-// tokens 55 / 41.  Three where four would leave more lanes without a head: 8 + 2 heads of
-// 32 in fp32, 19980 tokens, 14.7 us against 15.7.
+// tokens 55 / 41.  Three where four would leave more lanes without a head (us, three /
+// four, 48060 tokens, one axis): 8 + 2 heads of 32 in fp32 29 / 32, of 64 in fp16 33 / 37, 16 + 4 of 64 in
+// fp16 62 / 72; where they leave as many or more, four: 8 + 8 heads of 64 in fp16 61 / 41, 12 +
+// 4 of 32 in fp32 51 / 39, 16 + 4 of 64 in fp32 105 / 98.
 template <typename T, int LANES, bool WHOLE>
 void launch_unrolled(const NormRopeArgs& a, cudaStream_t st) {
     constexpr int GROUPS = 32 / LANES;
