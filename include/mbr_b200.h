@@ -319,7 +319,8 @@ typedef struct mbr_view {
 
 /* A rolling key/value cache.  Position p of a sequence lives in slot p while
  * p < sinks and in slot sinks + (p - sinks) % ring after that, so the first
- * `sinks` tokens stay and the newest `ring` others replace the older ones.
+ * `sinks` tokens stay and the newest `ring` others replace the older ones;
+ * ring >= 1, sinks + ring <= 2^30.
  * bits 0: k and v are [seqs][kv_heads][sinks + ring][dim_head] of dtype
  * (MBR_FP32 / MBR_FP16 / MBR_BF16), k_scale and v_scale are null.
  * bits 4 (MBR_FP16 / MBR_BF16, dim_head a multiple of 32): k and v hold one

@@ -15,7 +15,9 @@ namespace streamops {
 
 void check_cache_fields(const mbr_kv_cache& c) {
     MBR_CHECK(c.seqs >= 0 && c.kv_heads >= 0 && c.sinks >= 0, "kv cache: negative size");
-    MBR_CHECK(c.ring >= 1 && c.sinks < (1 << 30) && c.ring < (1 << 30), "kv cache: ring must be 1..2^30 - 1");
+    MBR_CHECK(c.ring >= 1, "kv cache: ring must be at least 1");
+    // a query's keys are counted in 32 bits, rounded up to whole copies
+    MBR_CHECK((int64_t)c.sinks + c.ring <= (1 << 30), "kv cache: sinks and ring must not exceed 2^30 together");
     MBR_CHECK(c.dtype == DT_F32 || c.dtype == DT_F16 || c.dtype == DT_BF16, "kv cache: dtype must be fp32, fp16 or bf16");
     MBR_CHECK(c.bits == 0 || c.bits == 4, "kv cache: bits must be 0 or 4");
     MBR_CHECK(c.dim_head >= 8 && c.dim_head <= 128 && c.dim_head % 8 == 0,
