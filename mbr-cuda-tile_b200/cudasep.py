@@ -311,12 +311,10 @@ def _workspace(n, device, stream):
 
 
 def _empty_on(stream, shape, dtype, device):
-    """An uninitialised output of a call on `stream` (None: the current one): that stream's memory, which the current
-    stream, whose work may read it, has to be done with before it is used again."""
+    """An uninitialised output of a call on `stream`: that stream's memory, which the current stream, whose work may read
+    it, has to be done with before it is used again."""
     import torch
 
-    if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
     with torch.cuda.stream(_torch_stream(stream, device)):
         t = torch.empty(shape, dtype=dtype, device=device)
     t.record_stream(torch.cuda.current_stream(device))
@@ -360,7 +358,8 @@ class KVCache:
 
     def new(self, shape, stream=None):
         """An uninitialised tensor of the cache's type on its device, the memory of `stream` (None: the current one)."""
-        return _empty_on(stream, shape, self.dtype, self.k.device)
+        t = self._k_scale if self._bits else self._k
+        return t.new_empty(shape) if stream is None else _empty_on(stream, shape, t.dtype, t.device)
 
     @classmethod
     def empty(cls, seqs, kv_heads, slots, dim_head, dtype, sinks=0, bits=0, device="cuda"):
