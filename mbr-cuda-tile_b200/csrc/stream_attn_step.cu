@@ -365,15 +365,17 @@ __global__ void __launch_bounds__(StepCfg<DP, Q4>::WARPS * 32, 1) attend_step_ke
             }
             if (Q4 || !CACHED) cp_async_commit();
         };
-        // The slot to be read next has landed; false (in every lane) if the wait for it ran out.  Then what else this
-        // warp has in flight (the copies before the `sent`-th, one a slot) is waited for too: nothing may land in
-        // shared memory that the warp has left.
-        auto landed = [&](int n, int sent) {
+        // The slot to be read next (copy n) has landed, and so has the one before it if `so_far` (this lane's); false (in
+        // every lane) if a wait ran out.  Then what else this warp has in flight (up to the `sent`-th copy, one a slot)
+        // is waited for too: nothing may land in shared memory that the warp has left.
+        auto arrived = [&] { return !CACHED || wait_bytes(bar + st * 8, parity, p.err); };
+        auto landed = [&](int n, int sent, bool so_far = true) {
             if constexpr (CACHED) {
-                if (!__all_sync(0xffffffffu, wait_bytes(bar + st * 8, parity, p.err))) {
-                    for (int i = n; i < min(sent, copies); ++i) {
-                        const int at = after(st, i - n);
-                        mbar_drain((uint64_t*)__cvta_shared_to_generic(bar + at * 8), parity ^ (at < st));
+                so_far &= arrived();
+                if (!__all_sync(0xffffffffu, so_far)) {
+                    for (int i = n - Q4; i < min(sent, copies); ++i) {
+                        const int x = st + i - n, at = x < 0 ? x + SLOTS : x >= SLOTS ? x - SLOTS : x;
+                        mbar_drain((uint64_t*)__cvta_shared_to_generic(bar + at * 8), parity ^ (at != x));
                     }
                     if (Q4) cp_async_wait<0>();
                     __syncwarp();
@@ -443,12 +445,14 @@ __global__ void __launch_bounds__(StepCfg<DP, Q4>::WARPS * 32, 1) attend_step_ke
         for (int n = 0; n < copies; n += 2) {
             // 16-bit rows: the keys' slot is refilled as soon as S is computed.  Codes: both slots serve two units.
             fetch(n + SLOTS - 1, after(st, SLOTS - 1));  // into the slot read last, while this one is worked on
-            if (!landed(n, n + SLOTS)) break;
+            bool keys = true;
+            if constexpr (Q4) keys = arrived();
+            else if (!landed(n, n + SLOTS)) break;
             const uint32_t k_slot = ring + st * Cfg::SLOT;
             uint32_t v_slot = 0;
             if constexpr (Q4) {
                 next();
-                if (!landed(n + 1, n + SLOTS)) break;
+                if (!landed(n + 1, n + SLOTS, keys)) break;
                 cp_async_wait<SLOTS - 2>();  // both slots' steps and offsets
                 __syncwarp();
                 v_slot = ring + st * Cfg::SLOT;

@@ -77,14 +77,14 @@ def step_group(items, slots, codes, seed, tired, warps=2, keeps_on=False, hasty=
             st = after(1)
             parity ^= st == 0
 
-        def landed(n, sent, copies):
+        def landed(n, sent, copies, so_far=True):
             nonlocal alive
-            ok = yield from cta.wait(bars[st], parity)
+            ok = (yield from cta.wait(bars[st], parity)) and so_far
             if not ok and not keeps_on:
                 alive = False
-                for i in range(n, min(sent, copies)):
-                    at = after(i - n)
-                    yield from cta.drain(bars[at], parity ^ (at < st), hasty)
+                for i in range(n - codes, min(sent, copies)):
+                    x = st + i - n
+                    yield from cta.drain(bars[x % slots], parity ^ (not 0 <= x < slots), hasty)
             return alive
 
         for it, n_copies in enumerate(items):
@@ -98,13 +98,18 @@ def step_group(items, slots, codes, seed, tired, warps=2, keeps_on=False, hasty=
                 fetch(n, after(n))
             for n in range(0, copies, 2):
                 fetch(n + slots - 1, after(slots - 1))
-                if not (yield from landed(n, n + slots, copies)):
-                    break
-                step()
-                if not codes:
+                if codes:  # keys and values are looked at together
+                    keys = yield from cta.wait(bars[st], parity)
+                    step()
+                    if not (yield from landed(n + 1, n + slots, copies, keys)):
+                        break
+                else:
+                    if not (yield from landed(n, n + slots, copies)):
+                        break
+                    step()
                     fetch(n + slots, after(slots - 1))
-                if not (yield from landed(n + 1, n + slots + (not codes), copies)):
-                    break
+                    if not (yield from landed(n + 1, n + slots + 1, copies)):
+                        break
                 step()
                 if codes:
                     fetch(n + slots, after(slots - 2))
