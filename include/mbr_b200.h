@@ -327,7 +327,7 @@ typedef struct mbr_view {
  * byte for two values, channel 2i in the low half of byte i; k_scale and
  * v_scale are [seqs][kv_heads][sinks + ring][dim_head / 32][2] of dtype, the
  * step s and offset m of each group of 32 channels: code c stands for
- * m + s * (c - 8), rounded to dtype. */
+ * m + s * (c - 8), rounded to dtype once. */
 typedef struct mbr_kv_cache {
     void* k;
     void* v;
@@ -360,8 +360,9 @@ MBR_API int mbr_op_qk_norm_rope(const mbr_view* q, const mbr_view* k, const mbr_
  * counts as `tokens`), into the cache; k, v [seqs][tokens][kv_heads][dim_head].
  * Of tokens that share a ring slot only the newest is written; negative
  * positions are left out.  4-bit groups: with T(x) the rounding to dtype, s =
- * T((max - min) / 15), m = T(min + 8 s), c = clamp(rint((x - m) / s) + 8, 0,
- * 15); a group whose range is not finite is NaN when read. */
+ * T((max - min) * (1 / 15)), m = T(min + 8 s), c = clamp(rint((x - m) * (1 / s))
+ * + 8, 0, 15), all in fp32 with each operation (1 / 15 and 1 / s too) rounded
+ * and none overflowing; codes 8 if s is 0.  A group whose range is not finite is NaN when read. */
 MBR_API int mbr_op_cache_append(const mbr_kv_cache* cache, const mbr_view* k, const mbr_view* v,
                                 const int32_t* d_pos, const int32_t* d_count, int64_t tokens, void* stream);
 

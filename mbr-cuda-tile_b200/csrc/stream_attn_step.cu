@@ -140,7 +140,9 @@ struct Widen<__nv_bfloat16> {
     uint32_t mask = held(0x000f000fu), base = held(0x43004300u), less = held(0xc308c308u);  // -136
 };
 // The two values that the codes at bits 4i and 16 + 4i of x stand for: code -
-// 8 (exact in 16 bits), times the step plus the offset in one rounding.
+// 8 (exact in 16 bits), times the step plus the offset in one rounding.  The code
+// becomes a number by the well-known way of setting it into the last bits of a
+// power of two's mantissa and subtracting that.
 // s, m: step and offset of both.
 __device__ __forceinline__ uint32_t masked(uint32_t x, uint32_t mask, uint32_t base) {
     uint32_t r;

@@ -3,11 +3,12 @@
 //
 // y = x * rsqrt(mean_d x^2 + eps) * gamma over one head of one token, then the
 // pair (2i, 2i+1) turned by the angle of its axis' position: every element is
-// read once and written once, so memory bounds it.  A group of lanes holds one
+// read once and written once, so memory is its floor.  A group of lanes holds one
 // head in registers (16 bytes a lane); the group's sum of squares is a shuffle
 // butterfly, in fp32 like everything up to the final rounding.  60 x 801 tokens
 // of 8 + 8 heads of 64 in fp16, two axes, read in place from a packed q|k|v
-// (197 MB): 41.6 us, 4.7 TB/s (the form for any layout: 260 us); 60 tokens 2.2 us.
+// (197 MB): 41.6 us, 4.7 TB/s (DRAM 41 % and issue slots 60 % busy: latency; the
+// form for any layout: 253 us); 60 tokens 2.2 us.
 // At fp32, heads of 32 and three axes the angles' loads and the instructions of
 // the turn weigh more: 51 MB in 14.7 us, 3.5 TB/s.
 #include <algorithm>
