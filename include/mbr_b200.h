@@ -422,7 +422,8 @@ MBR_API int mbr_op_cache_attention_workspace(const mbr_kv_cache* cache, int64_t 
  * graph replays, which neither look at the word nor clear it: with the stream
  * that was captured, once the replays have run.  mbr_op_stream_error_word gives
  * the word's address (host memory, 0: none, valid as long as the process), for
- * a look without waiting.  Words are kept by device and stream handle. */
+ * a look without waiting.  Words are kept by stream handle (the default
+ * streams' by device: the current one). */
 MBR_API int mbr_op_stream_check(void* stream);
 MBR_API int mbr_op_stream_error_word(void* stream, volatile int** word);
 

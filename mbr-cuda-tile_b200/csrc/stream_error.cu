@@ -30,10 +30,11 @@ Words& words() {
     return *w;
 }
 
-// The word of a stream of the current device, or null if it has none and `make` is false.
+// The word of a stream, or null if it has none and `make` is false.  A handle says which stream it is on any
+// device, but for the names of each device's default streams.
 int* word_of(cudaStream_t st, bool make) {
     if (st == cudaStreamLegacy) st = nullptr;  // two names of one stream
-    const int dev = stream_device();
+    const int dev = st == nullptr || st == cudaStreamPerThread ? stream_device() : -1;
     Words& w = words();
     const std::lock_guard<std::mutex> lock(w.mu);
     const auto at = w.of.find({dev, st});

@@ -412,7 +412,10 @@ def op_cache_attention(q, cache, length, left=-1, right=0, scale=0.0, gates=None
 def op_stream_check(stream=None):
     """Waits for the stream and raises MBRError if a kernel-side wait of an attention call above ran out on it: to be
     called after the last one, and after graph replays (with the stream that was captured)."""
-    _check(lib().mbr_op_stream_check(_stream(stream)))
+    import torch
+
+    with torch.cuda.device(stream.device if isinstance(stream, torch.cuda.Stream) else None):
+        _check(lib().mbr_op_stream_check(_stream(stream)))
 
 
 def op_stft(sig, hop=441, stream=None):
